@@ -472,6 +472,107 @@ typedef struct {
 
 int wzyb_embed_ple_f16(const wzyb_embed_ple_args* a, int64_t T, wzyb_stream_t stream);
 
+/* ============================================================================================
+ * Attention over the INT8 KV cache: a sliding window plus the first tokens, which stay visible (sinks).
+ * q [T, q_heads, head_dim] (fp16 for the _f16 calls, fp32 for _f32), already normed and rotated; query
+ * head h reads kv head h / (q_heads / kv_heads). Query t stands at p = (d_base_pos ? *d_base_pos : 0) +
+ * pos_offset + t and sees position j when
+ *   0 <= j <= p,  j < max_ctx,  (j < sinks or j > p - window),  and the chosen copy of the cache holds j.
+ * Call it after the T tokens' k, v have been appended with the same base: WZYB_KV_RING reads the ring, which
+ * holds the positions of the append's rule with end = base + T; WZYB_KV_FULL reads the full-context mirror,
+ * which holds all below max_ctx (the other copy's pointers may then be NULL). A window that is no longer
+ * than the ring (ring_cap - 4096 - T past the pinned cells) loses nothing. window = 0 leaves the sinks
+ * alone, sinks = 0 the window; a window >= max_ctx is plain causal attention.
+ *   x_j = scale * (q . k_j);  out = sum_j softmax(x)_j v_j;  lse[t, h] = ln sum_j exp(x_j)  (lse may be NULL)
+ * with k_j, v_j = code * scale of the cell's 64-element groups. A query that sees nothing gets out = 0 and
+ * lse = -inf. Cells that a query does not see never reach its result, whatever they hold.
+ * head_dim in {64, 128, 256}; q_heads a multiple of kv_heads, at most 256; kv_heads <= 64; T <= 2^22;
+ * max_ctx and ring_cap below 2^31; strides in elements. Cache codes and scales 16-byte aligned.
+ * workspace: wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim) bytes of device memory (0: none needed),
+ * 16-byte aligned, of no meaning between calls; calls on different streams need their own.
+ * ========================================================================================== */
+#define WZYB_KV_RING 0
+#define WZYB_KV_FULL 1
+typedef struct {
+    const void* q;
+    int q_heads;
+    int64_t q_head_stride;
+    int64_t q_row_stride;
+    void* out; /* [T, q_heads, head_dim], q's element type */
+    int64_t out_head_stride;
+    int64_t out_row_stride;
+    float* lse; /* [T, q_heads] or NULL */
+    const wzyb_kv_cache* cache;
+    int source; /* WZYB_KV_RING or WZYB_KV_FULL */
+    int kv_heads;
+    int head_dim;
+    const int32_t* d_base_pos;
+    int64_t pos_offset;
+    int64_t window;
+    int64_t sinks;
+    float scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} wzyb_kv_attn_args;
+int64_t wzyb_kv_attn_workspace(int64_t T, int q_heads, int kv_heads, int head_dim);
+int wzyb_kv_attn_f16(const wzyb_kv_attn_args* a, int64_t T, wzyb_stream_t stream);
+int wzyb_kv_attn_f32(const wzyb_kv_attn_args* a, int64_t T, wzyb_stream_t stream);
+/* Attention for a tree of drafted tokens. base = (d_base_pos ? *d_base_pos : 0) + pos_offset tokens are
+ * committed (positions 0 .. base - 1, the ring holding what it does with end = base). Node i < nodes stands
+ * at p_i = base + depth[i], sees the committed positions by the rule above with p = p_i, and the drafts
+ * j < nodes whose bit is set in its row of `mask` ([nodes, ceil(nodes / 32)] words, bit j % 32 of word j / 32;
+ * a node's own bit included by the caller). The drafts' k, v are the cells 0 .. nodes - 1 of the ring of
+ * `drafts`, a second cache of the same kv_heads and head_dim: append them there with
+ * wzyb_kv_append_int8_f32 (k rotated at p_i), and the accepted ones to the cache afterwards; the cells are
+ * quantised alike. nodes <= WZYB_TREE_MAX_NODES and <= drafts->ring_cap; depth [nodes]. Workspace as
+ * wzyb_kv_attn_workspace(nodes, ...). */
+#define WZYB_TREE_MAX_NODES 1024
+int wzyb_kv_tree_attn_f16(const wzyb_kv_attn_args* a, const wzyb_kv_cache* drafts, const uint32_t* mask,
+                          const int32_t* depth, int64_t nodes, wzyb_stream_t stream);
+int wzyb_kv_tree_attn_f32(const wzyb_kv_attn_args* a, const wzyb_kv_cache* drafts, const uint32_t* mask,
+                          const int32_t* depth, int64_t nodes, wzyb_stream_t stream);
+
+/* ============================================================================================
+ * The gated delta rule: the recurrence whose output wzyb_gdn_gated_norm_* norms and gates. Per value head
+ * (its q, k head is h / (v_heads / k_heads)), with the state S [v, k] (S[j] the k-vector of value column j):
+ *   S <- e^(g_t) S;  d = beta_t (v_t - S k_t);  S <- S + d k_t^T;  o_t = scale * S q_t
+ * q, k [T, k_heads, head_dim], v, o [T, v_heads, head_dim] (fp16 for _f16, fp32 for _f32; heads contiguous,
+ * tokens *_row_stride elements apart, so q, k, v may be slices of one projection); g (log decay, usually
+ * <= 0, -inf resets) and beta [T, v_heads] fp32. qk_l2norm != 0 norms q and k first:
+ * x * rsqrt(sum x^2 + l2_eps). state_in [v_heads, head_dim, head_dim] fp32 or NULL (zeros), state_out the
+ * state after the last token (the same buffer as state_in is allowed); state_snaps [T, v_heads, head_dim,
+ * head_dim] or NULL: the state after every token, for taking back rejected drafts. head_dim in {64, 128};
+ * v_heads a multiple of k_heads, at most 1024; T = 0 copies the state. o must not overlap the inputs.
+ * workspace: wzyb_gdn_delta_rule_workspace(T, k_heads, v_heads, head_dim) bytes of device memory (0: none),
+ * 16-byte aligned, of no meaning between calls.
+ * ========================================================================================== */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_row_stride;
+    int64_t k_row_stride;
+    int64_t v_row_stride;
+    const float* g;
+    const float* beta;
+    const float* state_in;
+    float* state_out;
+    float* state_snaps;
+    void* o;
+    int64_t o_row_stride;
+    int k_heads;
+    int v_heads;
+    int head_dim;
+    float scale;
+    int qk_l2norm;
+    float l2_eps;
+    void* workspace;
+    int64_t workspace_bytes;
+} wzyb_gdn_delta_args;
+int64_t wzyb_gdn_delta_rule_workspace(int64_t T, int k_heads, int v_heads, int head_dim);
+int wzyb_gdn_delta_rule_f16(const wzyb_gdn_delta_args* a, int64_t T, wzyb_stream_t stream);
+int wzyb_gdn_delta_rule_f32(const wzyb_gdn_delta_args* a, int64_t T, wzyb_stream_t stream);
+
 /* Token-row sharding for G independent GPUs (no collective): rank r gets rows
  * [row0, row0 + rows) of a contiguous ceil(total/G) split. */
 int wzyb_shard_rows(int64_t total, int world, int rank, int64_t* row0, int64_t* rows);

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_double, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -26,6 +27,8 @@ PLE_EOS_DEFAULT = 248044
 FAM_NORM, FAM_HEAD_ROPE, FAM_GDN, FAM_SWIGLU, FAM_GATHER, FAM_BUNDLE, FAM_KV = 0, 1, 2, 3, 4, 5, 6
 VARIANT_AUTO, VARIANT_RING, VARIANT_DIRECT, VARIANT_ASYNC, VARIANT_WIDE, VARIANT_PAIR = 0, 1, 2, 3, 4, 5
 VARIANT_SPLIT = 6
+KV_RING, KV_FULL = 0, 1
+TREE_MAX_NODES = 1024
 
 
 class WzybError(RuntimeError):
@@ -125,6 +128,63 @@ class EmbedPleArgs(ctypes.Structure):
     ]
 
 
+class KvAttnArgs(ctypes.Structure):
+    """wzyb_kv_attn_args."""
+    _fields_ = [
+        ("q", c_void_p),
+        ("q_heads", c_int),
+        ("q_head_stride", c_int64),
+        ("q_row_stride", c_int64),
+        ("out", c_void_p),
+        ("out_head_stride", c_int64),
+        ("out_row_stride", c_int64),
+        ("lse", c_void_p),
+        ("cache", POINTER(KvCache)),
+        ("source", c_int),
+        ("kv_heads", c_int),
+        ("head_dim", c_int),
+        ("d_base_pos", c_void_p),
+        ("pos_offset", c_int64),
+        ("window", c_int64),
+        ("sinks", c_int64),
+        ("scale", c_float),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class GdnDeltaArgs(ctypes.Structure):
+    """wzyb_gdn_delta_args."""
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("q_row_stride", c_int64),
+        ("k_row_stride", c_int64),
+        ("v_row_stride", c_int64),
+        ("g", c_void_p),
+        ("beta", c_void_p),
+        ("state_in", c_void_p),
+        ("state_out", c_void_p),
+        ("state_snaps", c_void_p),
+        ("o", c_void_p),
+        ("o_row_stride", c_int64),
+        ("k_heads", c_int),
+        ("v_heads", c_int),
+        ("head_dim", c_int),
+        ("scale", c_float),
+        ("qk_l2norm", c_int),
+        ("l2_eps", c_float),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+# The same structs packed in one call (native alignment): a decoded token's launches are short enough for
+# the time of setting twenty ctypes fields to show.
+_KV_ATTN_PACK = struct.Struct("@PiqqPqqPPiiiPqqqfPq").pack
+_GDN_DELTA_PACK = struct.Struct("@PPPqqqPPPPPPqiiififPq").pack
+
 P = c_void_p
 S = c_void_p  # cudaStream_t
 _SIGS = {
@@ -203,6 +263,14 @@ _SIGS = {
     "wzyb_attn_prep_f16": (c_int, [POINTER(AttnPrepArgs), c_int64, S]),
     "wzyb_act_f16": (c_int, [POINTER(ActArgs), c_int64, S]),
     "wzyb_embed_ple_f16": (c_int, [POINTER(EmbedPleArgs), c_int64, S]),
+    "wzyb_kv_attn_workspace": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "wzyb_kv_attn_f16": (c_int, [P, c_int64, S]),
+    "wzyb_kv_attn_f32": (c_int, [P, c_int64, S]),
+    "wzyb_kv_tree_attn_f16": (c_int, [P, P, P, P, c_int64, S]),
+    "wzyb_kv_tree_attn_f32": (c_int, [P, P, P, P, c_int64, S]),
+    "wzyb_gdn_delta_rule_workspace": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "wzyb_gdn_delta_rule_f16": (c_int, [P, c_int64, S]),
+    "wzyb_gdn_delta_rule_f32": (c_int, [P, c_int64, S]),
     "wzyb_shard_rows": (c_int, [c_int64, c_int, c_int, POINTER(c_int64), POINTER(c_int64)]),
     "wzyb_ple_halo": (c_int, [POINTER(c_int32), c_int64, POINTER(c_int32), POINTER(c_int32)]),
     "wzyb_prepare_device": (c_int, []),
@@ -404,6 +472,127 @@ def k_rope_kv_append(k, k_gamma, v, cos_tab, sin_tab, T, kv_heads, head_dim, cac
         call("wzyb_qk_rope_kv_append_f16" if f16 else "wzyb_qk_rope_kv_append_f32", ctypes.byref(q), *args)
     else:
         call("wzyb_k_rope_kv_append_f16" if f16 else "wzyb_k_rope_kv_append_f32", *args)
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _raw_stream(stream, index):
+    """The cudaStream_t of `stream`, or of the current stream of device `index`."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def kv_attn_workspace_bytes(T, q_heads, kv_heads, head_dim) -> int:
+    """Bytes of workspace of kv_attn (T tokens) or kv_tree_attn (T nodes); 0 when none is needed."""
+    return int(lib().wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim))
+
+
+def _elem_size(q):
+    """2 for float16, 4 for float32 tensors on a CUDA device."""
+    size = {"torch.float16": 2, "torch.float32": 4}.get(str(q.dtype))
+    _need(size is not None and q.is_cuda, "expected float16 or float32 tensors on a CUDA device")
+    return size
+
+
+def _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace):
+    import torch
+
+    T, q_heads, head_dim = shape = q.shape
+    qr, qh, qe = q.stride()
+    orow, oh, oe = out.stride()
+    _need(out.shape == shape and out.dtype == q.dtype and out.device == q.device, "out: expected q's shape, type and device")
+    _need(qe == 1 and oe == 1, "q and out: the head dimension must be contiguous")
+    _need(d_base_pos is None or (d_base_pos.dtype == torch.int32 and d_base_pos.is_cuda), "d_base_pos: expected int32 on the device")
+    if lse is not None:
+        _need(lse.shape == shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous() and lse.is_cuda,
+              "lse: expected a contiguous float32 [T, q_heads] tensor")
+    return _KV_ATTN_PACK(q.data_ptr(), q_heads, qh, qr, out.data_ptr(), oh, orow, 0 if lse is None else lse.data_ptr(),
+                         ctypes.addressof(cache), source, kv_heads, head_dim,
+                         0 if d_base_pos is None else d_base_pos.data_ptr(), pos_offset, window, sinks,
+                         head_dim**-0.5 if scale is None else scale, *_workspace(workspace))
+
+
+def _workspace(ws):
+    if ws is None:
+        return 0, 0
+    _need(ws.is_contiguous() and ws.is_cuda, "workspace must be contiguous and on the device")
+    return ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+def kv_attn(q, out, cache: KvCache, kv_heads, window, sinks=0, scale=None, source=KV_RING, d_base_pos=None,
+            pos_offset=0, lse=None, workspace=None, stream=None):
+    """Attention of the T tokens of q [T, q_heads, head_dim] (fp16 or fp32, any head and token stride) over the
+    INT8 cache they were appended to: each sees the last `window` positions up to its own and the first
+    `sinks`. scale defaults to head_dim**-0.5; workspace: kv_attn_workspace_bytes(...) bytes on the device."""
+    f16 = _elem_size(q) == 2
+    args = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    fn = "wzyb_kv_attn_f16" if f16 else "wzyb_kv_attn_f32"
+    rc = getattr(lib(), fn)(args, q.shape[0], _raw_stream(stream, q.device.index))
+    if rc:
+        check(fn, rc)
+
+
+def kv_tree_attn(q, out, cache: KvCache, drafts: KvCache, mask, kv_heads, window, depth, sinks=0, scale=None,
+                 source=KV_RING, d_base_pos=None, pos_offset=0, lse=None, workspace=None, stream=None):
+    """Attention of drafted nodes q [N, q_heads, head_dim]: node i stands at base + depth[i] over the `base`
+    committed tokens of the cache and sees the drafts whose bit is set in mask [N, ceil(N / 32)] (int32 words);
+    the drafts' k, v are cells 0..N-1 of the `drafts` ring."""
+    import torch
+
+    f16 = _elem_size(q) == 2
+    args = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    n = q.shape[0]
+    _need(mask.shape == (n, (n + 31) // 32) and mask.dtype == torch.int32 and mask.is_contiguous() and mask.is_cuda,
+          "mask: expected a contiguous int32 [N, ceil(N / 32)] tensor")
+    _need(depth.shape == (n,) and depth.dtype == torch.int32 and depth.is_contiguous() and depth.is_cuda,
+          "depth: expected a contiguous int32 [N] tensor")
+    fn = "wzyb_kv_tree_attn_f16" if f16 else "wzyb_kv_tree_attn_f32"
+    rc = getattr(lib(), fn)(args, ctypes.addressof(drafts), mask.data_ptr(), depth.data_ptr(), n,
+                            _raw_stream(stream, q.device.index))
+    if rc:
+        check(fn, rc)
+
+
+def gdn_delta_rule_workspace_bytes(T, k_heads, v_heads, head_dim=128) -> int:
+    """Bytes of workspace of gdn_delta_rule; 0 when none is needed."""
+    return int(lib().wzyb_gdn_delta_rule_workspace(T, k_heads, v_heads, head_dim))
+
+
+def gdn_delta_rule(q, k, v, g, beta, o, state_out, state_in=None, state_snaps=None, scale=None, qk_l2norm=True,
+                   l2_eps=1e-6, workspace=None, stream=None):
+    """The gated delta rule over q, k [T, k_heads, d], v, o [T, v_heads, d] (fp16 or fp32; token strides free),
+    g, beta [T, v_heads] fp32, states [v_heads, d (v), d (k)] fp32 (state_in None: zeros; may be state_out).
+    state_snaps [T, v_heads, d, d]: the state after every token. scale defaults to d**-0.5."""
+    import torch
+
+    f16 = _elem_size(q) == 2
+    T, k_heads, d = q.shape
+    v_heads = v.shape[1]
+    dt, f32, st = q.dtype, torch.float32, (v_heads, d, d)
+    strides = []
+    for t, h in ((q, k_heads), (k, k_heads), (v, v_heads), (o, v_heads)):
+        row, head, elem = t.stride()
+        _need(t.dtype == dt and t.shape == (T, h, d) and t.is_cuda, "q, k [T, k_heads, d], v, o [T, v_heads, d]: shapes or types differ")
+        _need(elem == 1 and (head == d or h == 1), "q, k, v, o: the heads of a token must be contiguous")
+        strides.append(row)
+    for t, shape in ((g, (T, v_heads)), (beta, (T, v_heads)), (state_out, st), (state_in, st), (state_snaps, (T, *st))):
+        _need(t is None or (t.dtype == f32 and t.shape == shape and t.is_contiguous() and t.is_cuda),
+              "g, beta and the states: expected contiguous float32 tensors of their shapes")
+    args = _GDN_DELTA_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides[:3], g.data_ptr(), beta.data_ptr(),
+                           0 if state_in is None else state_in.data_ptr(), state_out.data_ptr(),
+                           0 if state_snaps is None else state_snaps.data_ptr(), o.data_ptr(), strides[3], k_heads,
+                           v_heads, d, d**-0.5 if scale is None else scale, 1 if qk_l2norm else 0, l2_eps,
+                           *_workspace(workspace))
+    fn = "wzyb_gdn_delta_rule_f16" if f16 else "wzyb_gdn_delta_rule_f32"
+    rc = getattr(lib(), fn)(args, T, _raw_stream(stream, q.device.index))
+    if rc:
+        check(fn, rc)
 
 
 def rope_table(cos_tab, sin_tab, rows, rot_dims=64, theta=1e7, stream=None):
