@@ -187,6 +187,655 @@ __global__ void __launch_bounds__(256) gdn_recurrent_kernel(const GdnDeltaArgs a
             make_float4(s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y);
 }
 
+// ----------------------------------------------------------------------------------------------------
+// The chunked form, for many tokens. With G the running sum of g inside a chunk of 64 tokens, k^ = rk k,
+// q^ = rq q (norms as row factors, so that fp16 inputs stay as they are) and S the state at its start:
+//   A_ij = beta_i e^(G_i - G_j) k^_i.k^_j  (i > j),     T = (I + A)^-1
+//   d = T diag(beta) (V - diag(e^G) K^ S),              o = scale (diag(e^G) Q^ S + tril(e^(G_i - G_j) q^_i.k^_j) d)
+//   S <- e^(G_64) S + sum_j e^(G_64 - G_j) k^_j d_j
+// T, the masked score matrix P and the row factors do not depend on S: gdn_chunk_prep_kernel makes them for
+// all chunks of a segment at once. gdn_chunk_scan_kernel then walks the chunks; its products with S, d and T
+// run on the tensor cores (mma m16n8k16).
+//
+// Precision. The state has to stay an fp32 state, and fp16 products of a rounded S would leave 2^-12 in it. So every
+// fp32 operand enters as two fp16 parts, x 2^-e = hi + 2^-11 lo (lo stored 2^11 times as large, so it is not cut
+// off), and a product takes hi*hi, hi*lo and, where both operands are split, lo*hi: 22 bits. k and q of fp16
+// calls are one part and exact. The exponents e are per value column (columns never mix), P and T have one each.
+// Running sums never live in a tensor-core accumulator for longer than a chunk (its sums are cut off towards
+// zero): S is updated in fp32 registers.
+// ----------------------------------------------------------------------------------------------------
+constexpr int kGdnChunk = 64;
+constexpr float kGdnLo = 2048.f;
+
+// A (chunk, value head)'s part of the workspace. Matrices as mma A fragments, 16 bytes per lane: fragment
+// (m-tile i, k-step j <= i) at index i * (i + 1) / 2 + j, 512 bytes each.
+template <bool kSplit>
+struct GdnChunkData {
+    uint4 t_hi[10][32], t_lo[10][32];
+    uint4 p[kSplit ? 20 : 10][32];  // split: hi parts, then lo parts
+    float a[64], b[64], c[64];      // row factors of K S, Q S and d
+    float decay, t_up, p_up, pad;   // e^(G_64), 2^e of T and of P
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+    mma_f16(d, x, b0, b1);
+}
+__device__ __forceinline__ void gdn_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn((x - f.x) * kGdnLo, (y - f.y) * kGdnLo);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// e with |x| < 2^e for a finite x, within [-100, 120]
+__device__ __forceinline__ int gdn_exp(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 0xFF) - 126;
+    return e < -100 ? -100 : (e > 120 ? 120 : e);
+}
+__device__ __forceinline__ float gdn_exp2i(int e) { return __int_as_float((e + 127) << 23); }
+
+struct GdnPrepArgs {
+    GdnDeltaArgs x;
+    int64_t t0;      // first token of the segment
+    uint8_t* data;   // [chunks, v_heads] GdnChunkData
+    __half* kq;      // fp32 calls: [chunks, k_heads, 4 (k hi, k lo, q hi, q lo), 64, HD]
+};
+
+template <typename T, int HD>
+struct GdnPrepSmem {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kLd = HD + 8;
+    __half k[kSplit ? 2 : 1][64 * kLd], q[kSplit ? 2 : 1][64 * kLd];
+    float A[64][68];
+    float tm[64][68];
+    float rk[64], rq[64], beta[64], ghi[64], glo[64];
+    unsigned int amax[2];
+};
+
+// One CTA of 4 warps per (chunk, k head), over the value heads that share it. Warp w owns rows 16w .. 16w+15.
+// T by blocks of 16: a diagonal block's inverse by forward substitution (a lane per column), then the column
+// block j below it by warp j: T_ij = -T_ii sum_k A_ik T_kj, fp32 FMA.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p) {
+    pdl_begin();
+    using S = GdnPrepSmem<T, HD>;
+    constexpr bool kSplit = S::kSplit;
+    constexpr int kLd = S::kLd;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    S& sm = *reinterpret_cast<S*>(smem_raw);
+    const GdnDeltaArgs& a = p.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int chunk = blockIdx.x / a.k_heads, hk = blockIdx.x % a.k_heads;
+    const int64_t tok0 = p.t0 + (int64_t)chunk * kGdnChunk;
+    const int n = (int)(a.T - tok0 < kGdnChunk ? a.T - tok0 : kGdnChunk);
+    constexpr int kL = HD / 8;  // lanes per row
+
+    for (int r0 = 0; r0 < 64; r0 += 128 / kL) {
+        const int r = r0 + tid / kL, col = (tid % kL) * 8;
+        float x[2][8];
+        float f[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const T* src = static_cast<const T*>(m ? a.q : a.k) + (tok0 + r) * (m ? a.q_row : a.k_row) + hk * HD + col;
+            if (r < n) {
+                Vec8<T>::load_ro(src, x[m]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[m][i] = 0.f;
+            }
+            float ss = 0.f, am = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ss = fmaf(x[m][i], x[m][i], ss);
+                am = fmaxf(am, fabsf(x[m][i]));
+            }
+            ss = group_sum<kL>(ss);
+            f[m] = r < n ? (a.l2norm ? rsqrtf(ss + a.l2_eps) : 1.f) : 0.f;
+            __half* const hi = (m ? sm.q[0] : sm.k[0]) + r * kLd + col;
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int o = kL / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+                const int e = am == 0.f ? 0 : gdn_exp(am);
+                const float down = gdn_exp2i(-e);
+                f[m] *= gdn_exp2i(e);
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gdn_split(x[m][2 * i] * down, x[m][2 * i + 1] * down, h[i], l[i]);
+                const uint4 vh = make_uint4(h[0], h[1], h[2], h[3]), vl = make_uint4(l[0], l[1], l[2], l[3]);
+                *reinterpret_cast<uint4*>(hi) = vh;
+                *reinterpret_cast<uint4*>((m ? sm.q[kSplit] : sm.k[kSplit]) + r * kLd + col) = vl;
+                __half* const dst = p.kq + ((int64_t)chunk * a.k_heads + hk) * (4 * 64 * HD) + m * (2 * 64 * HD) + r * HD + col;
+                *reinterpret_cast<uint4*>(dst) = vh;
+                *reinterpret_cast<uint4*>(dst + 64 * HD) = vl;
+            } else {
+                *reinterpret_cast<uint4*>(hi) = Vec8<__half>::from_f32(x[m]);
+            }
+        }
+        if (col == 0) {
+            sm.rk[r] = f[0];
+            sm.rq[r] = f[1] * a.scale;
+        }
+    }
+    __syncthreads();
+
+    // raw k.k and q.k of this warp's rows, columns up to the diagonal block
+    float kk[8][4], qk[8][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float (&acc)[8][4] = m ? qk : kk;
+        const __half* const xh = m ? sm.q[0] : sm.k[0];
+        const __half* const xl = m ? sm.q[kSplit] : sm.k[kSplit];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
+        const int arow = warp * 16 + (lane & 15), acol = (lane >> 4) * 8;
+        const int brow = (lane & 7) + ((lane >> 4) << 3), bcol = ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int part = kSplit ? 1 : 0; part >= 0; --part) {
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                uint32_t fa[4], fl[4];
+                ldmatrix_x4(fa, xh + arow * kLd + ks * 16 + acol);
+                if (part == 1) ldmatrix_x4(fl, xl + arow * kLd + ks * 16 + acol);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i > warp) break;  // warp-uniform
+                    uint32_t fb[4];
+                    if (part == 1) {
+                        ldmatrix_x4(fb, sm.k[kSplit] + (i * 16 + brow) * kLd + ks * 16 + bcol);
+                        mma_f16(acc[2 * i], fa, fb[0], fb[1]);
+                        mma_f16(acc[2 * i + 1], fa, fb[2], fb[3]);
+                    }
+                    ldmatrix_x4(fb, sm.k[0] + (i * 16 + brow) * kLd + ks * 16 + bcol);
+                    if (part == 1) {
+                        mma_f16(acc[2 * i], fl, fb[0], fb[1]);
+                        mma_f16(acc[2 * i + 1], fl, fb[2], fb[3]);
+                    } else {
+                        mma_f16(acc[2 * i], fa, fb[0], fb[1]);
+                        mma_f16(acc[2 * i + 1], fa, fb[2], fb[3]);
+                    }
+                }
+            }
+            if (part == 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][c] *= 1.f / kGdnLo;
+            }
+        }
+    }
+
+    const int per = a.v_heads / a.k_heads;
+    for (int hv = 0; hv < per; ++hv) {
+        const int h = hk * per + hv;
+        GdnChunkData<kSplit>& out =
+            reinterpret_cast<GdnChunkData<kSplit>*>(p.data)[(int64_t)chunk * a.v_heads + h];
+        if (warp == 0) {
+            // running sums in fp64, held as two fp32 parts in log2 units: differences of close tokens keep their
+            // precision after strong decays. A decay below e^-120 is 0 in fp32 either way (so -inf is as well).
+            double s0 = 0., s1 = 0.;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 2 * lane + i;
+                float x = 0.f, b = 0.f;
+                if (t < n) {
+                    x = a.g[(tok0 + t) * a.v_heads + h];
+                    b = a.beta[(tok0 + t) * a.v_heads + h];
+                    x = x < -120.f ? -120.f : x;
+                }
+                sm.beta[t] = b;
+                (i ? s1 : s0) = (double)x * 1.4426950408889634;
+            }
+            s1 += s0;
+            double run = s1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += y;
+            }
+            s0 += run - s1;
+            s1 = run;
+            sm.ghi[2 * lane] = (float)s0;
+            sm.glo[2 * lane] = (float)(s0 - (float)s0);
+            sm.ghi[2 * lane + 1] = (float)s1;
+            sm.glo[2 * lane + 1] = (float)(s1 - (float)s1);
+            if (lane < 2) sm.amax[lane] = 0u;
+        }
+        __syncthreads();
+        float pv[8][4];
+        float p_max = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i > 2 * warp + 1) break;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = warp * 16 + g + (c >> 1) * 8, col = i * 8 + 2 * t4 + (c & 1);
+                const float d = ex2_approx((sm.ghi[r] - sm.ghi[col]) + (sm.glo[r] - sm.glo[col]));
+                sm.A[r][col] = r > col ? sm.beta[r] * (kk[i][c] * (sm.rk[r] * sm.rk[col]) * d) : 0.f;
+                pv[i][c] = r >= col ? qk[i][c] * (sm.rq[r] * sm.rk[col]) * d : 0.f;
+                p_max = fmaxf(p_max, fabsf(pv[i][c]));
+            }
+        }
+        if (tid < 64) {
+            const float e = ex2_approx(sm.ghi[tid] + sm.glo[tid]);
+            out.a[tid] = sm.rk[tid] * e;
+            out.b[tid] = sm.rq[tid] * e;
+            out.c[tid] = sm.rk[tid] * ex2_approx((sm.ghi[63] - sm.ghi[tid]) + (sm.glo[63] - sm.glo[tid]));
+        }
+        __syncwarp();
+        {  // inverse of the diagonal block: lane = column (the upper 16 lanes repeat the lower)
+            const int b0 = warp * 16, j = lane & 15;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float s = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (k < i) s = fmaf(sm.A[b0 + i][b0 + k], x[k], s);
+                x[i] = (i == j ? 1.f : 0.f) - s;
+            }
+            if (lane < 16) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sm.tm[b0 + i][b0 + j] = x[i];
+            }
+        }
+        __syncthreads();
+        {  // the blocks below it: lane = 2 rows x 4 columns
+            const int rr = (lane >> 2) * 2, cc = warp * 16 + (lane & 3) * 4;
+            for (int i = warp + 1; i < 4; ++i) {
+                float y[2][4] = {};
+                for (int k = warp; k < i; ++k) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float4 b = *reinterpret_cast<const float4*>(&sm.tm[k * 16 + e][cc]);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float x = sm.A[i * 16 + rr + r][k * 16 + e];
+                            y[r][0] = fmaf(x, b.x, y[r][0]);
+                            y[r][1] = fmaf(x, b.y, y[r][1]);
+                            y[r][2] = fmaf(x, b.z, y[r][2]);
+                            y[r][3] = fmaf(x, b.w, y[r][3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    *reinterpret_cast<float4*>(&sm.tm[i * 16 + rr + r][cc]) = make_float4(y[r][0], y[r][1], y[r][2], y[r][3]);
+                __syncwarp();
+                float z[2][4] = {};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float4 b = *reinterpret_cast<const float4*>(&sm.tm[i * 16 + e][cc]);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float x = sm.tm[i * 16 + rr + r][i * 16 + e];
+                        z[r][0] = fmaf(x, b.x, z[r][0]);
+                        z[r][1] = fmaf(x, b.y, z[r][1]);
+                        z[r][2] = fmaf(x, b.z, z[r][2]);
+                        z[r][3] = fmaf(x, b.w, z[r][3]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    *reinterpret_cast<float4*>(&sm.tm[i * 16 + rr + r][cc]) = make_float4(-z[r][0], -z[r][1], -z[r][2], -z[r][3]);
+                __syncwarp();
+            }
+        }
+        __syncthreads();
+        // T diag(beta) and P as fragments, scaled down only where they pass fp16's range
+        float tv[8][4];
+        float t_max = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i > 2 * warp + 1) break;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = warp * 16 + g + (c >> 1) * 8, col = i * 8 + 2 * t4 + (c & 1);
+                tv[i][c] = sm.tm[r][col] * sm.beta[col];
+                t_max = fmaxf(t_max, fabsf(tv[i][c]));
+            }
+        }
+        const unsigned int tb = __reduce_max_sync(0xffffffffu, __float_as_uint(t_max));
+        const unsigned int pb = __reduce_max_sync(0xffffffffu, __float_as_uint(p_max));
+        if (lane == 0) {
+            atomicMax(&sm.amax[0], tb);
+            atomicMax(&sm.amax[1], pb);
+        }
+        __syncthreads();
+        int et = gdn_exp(__uint_as_float(sm.amax[0])) - 14, ep = gdn_exp(__uint_as_float(sm.amax[1])) - 14;
+        et = et < 0 ? 0 : et;
+        ep = ep < 0 ? 0 : ep;
+        const float td = gdn_exp2i(-et), pd = gdn_exp2i(-ep);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > warp) break;
+            const int at = warp * (warp + 1) / 2 + j;
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                gdn_split(tv[2 * j + b][0] * td, tv[2 * j + b][1] * td, h[2 * b], l[2 * b]);
+                gdn_split(tv[2 * j + b][2] * td, tv[2 * j + b][3] * td, h[2 * b + 1], l[2 * b + 1]);
+            }
+            out.t_hi[at][lane] = make_uint4(h[0], h[1], h[2], h[3]);
+            out.t_lo[at][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                gdn_split(pv[2 * j + b][0] * pd, pv[2 * j + b][1] * pd, h[2 * b], l[2 * b]);
+                gdn_split(pv[2 * j + b][2] * pd, pv[2 * j + b][3] * pd, h[2 * b + 1], l[2 * b + 1]);
+            }
+            out.p[at][lane] = make_uint4(h[0], h[1], h[2], h[3]);
+            if constexpr (kSplit) out.p[10 + at][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+        if (tid == 0) {
+            out.decay = ex2_approx(sm.ghi[63] + sm.glo[63]);
+            out.t_up = gdn_exp2i(et);
+            out.p_up = gdn_exp2i(ep);
+            out.pad = 0.f;
+        }
+        __syncthreads();
+    }
+}
+
+struct GdnScanArgs {
+    GdnDeltaArgs x;
+    int64_t t0, t1;  // the segment's tokens
+    const float* state_in;
+    const uint8_t* data;
+    const __half* kq;
+};
+
+template <typename T, int HD>
+struct GdnScanStage {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kLd = HD + 8, kVLd = 32 + 16 / sizeof(T);
+    __half k[kSplit ? 2 : 1][64 * kLd], q[kSplit ? 2 : 1][64 * kLd];
+    T v[64 * kVLd];
+    GdnChunkData<kSplit> d;
+};
+
+// Two column exponents per lane (columns 2*t4, 2*t4 + 1 of its warp), alike over the lanes of a column: values
+// scaled by 2^-e stay below 2^14. `force` sets them anew (every 16 chunks, so they follow a shrinking state
+// down too); otherwise they move only when a value would pass 2^14.
+template <int N>
+__device__ __forceinline__ void gdn_col_exp(const float (&x)[N][4], int (&e)[2], bool force) {
+    float m[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m[c & 1] = fmaxf(m[c & 1], fabsf(x[i][c]));
+    const bool over = m[0] * gdn_exp2i(-e[0]) > 16384.f || m[1] * gdn_exp2i(-e[1]) > 16384.f;
+    if (__any_sync(0xffffffffu, over) || force) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+            if (force || m[i] * gdn_exp2i(-e[i]) > 16384.f) {
+                const int n = gdn_exp(m[i]) - 8;
+                e[i] = n < -100 ? -100 : n;
+            }
+        }
+    }
+}
+
+// Accumulator layout (rows g, g + 8 of each 16-row tile; columns 2*t4, 2*t4 + 1) to the second operand's (16 rows
+// per step, columns g): packed fp16 pairs through 8x8 register transposes.
+template <int N>
+__device__ __forceinline__ void gdn_operand(const float (&x)[N][4], const int (&e)[2], uint32_t (&hi)[N][2],
+                                            uint32_t (&lo)[N][2]) {
+    const float d0 = gdn_exp2i(-e[0]), d1 = gdn_exp2i(-e[1]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            uint32_t h, l;
+            gdn_split(x[i][2 * b] * d0, x[i][2 * b + 1] * d1, h, l);
+            hi[i][b] = transpose8(h);
+            lo[i][b] = transpose8(l);
+        }
+}
+
+// One warp owns 8 value columns of a head from the first chunk to the last: its part of S stays in its
+// registers as fp32 accumulator tiles, and S, X = V - e^G K S and d = T X pass from product to product inside the
+// warp (columns never mix), so the chunk's chain needs no barrier. The four warps of a CTA share the
+// chunk's K, Q, T and P in shared memory, fetched by cp.async while the chunk before is worked through.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
+    pdl_begin();
+    using Stage = GdnScanStage<T, HD>;
+    constexpr bool kSplit = Stage::kSplit;
+    constexpr int kLd = Stage::kLd, kVLd = Stage::kVLd, kM = HD / 16;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Stage* const st = reinterpret_cast<Stage*>(smem_raw);
+    const GdnDeltaArgs& a = p.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int h = blockIdx.x / (HD / 32), c0 = (blockIdx.x % (HD / 32)) * 32;
+    const int hk = h / (a.v_heads / a.k_heads);
+    const int chunks = (int)((p.t1 - p.t0 + kGdnChunk - 1) / kGdnChunk);
+
+    auto fetch = [&](int ch) {
+        Stage& s = st[ch & 1];
+        const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
+        const int n = (int)(p.t1 - tok0 < kGdnChunk ? p.t1 - tok0 : kGdnChunk);
+        constexpr int kRowChunks = HD / 8;
+        if constexpr (kSplit) {
+            const __half* const src = p.kq + ((int64_t)ch * a.k_heads + hk) * (4 * 64 * HD);
+#pragma unroll 4
+            for (int i = tid; i < 4 * 64 * kRowChunks; i += 128) {
+                const int m = i / (64 * kRowChunks), r = (i / kRowChunks) % 64, c = (i % kRowChunks) * 8;
+                __half* const base = m < 2 ? s.k[m & 1] : s.q[m & 1];
+                cp_async16(base + r * kLd + c, src + (m * 64 + r) * HD + c);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < 2 * 64 * kRowChunks; i += 128) {
+                const int m = i / (64 * kRowChunks), r = (i / kRowChunks) % 64, c = (i % kRowChunks) * 8;
+                __half* const dst = (m ? s.q[0] : s.k[0]) + r * kLd + c;
+                const __half* const src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r) * (m ? a.q_row : a.k_row) + hk * HD + c;
+                if (r < n)
+                    cp_async16(dst, src);
+                else
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        constexpr int kVC = 32 * sizeof(T) / 16, kVE = 16 / sizeof(T);
+#pragma unroll
+        for (int i = tid; i < 64 * kVC; i += 128) {
+            const int r = i / kVC, c = (i % kVC) * kVE;
+            T* const dst = s.v + r * kVLd + c;
+            if (r < n)
+                cp_async16(dst, static_cast<const T*>(a.v) + (tok0 + r) * a.v_row + h * HD + c0 + c);
+            else
+                *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+        }
+        const uint4* const src = reinterpret_cast<const uint4*>(p.data + ((int64_t)ch * a.v_heads + h) * sizeof(GdnChunkData<kSplit>));
+        uint4* const dst = reinterpret_cast<uint4*>(&s.d);
+#pragma unroll 4
+        for (int i = tid; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 128) cp_async16(dst + i, src + i);
+        cp_async_commit();
+    };
+
+    const int col = c0 + warp * 8 + 2 * t4;  // this lane's columns col, col + 1
+    float s[kM][4];  // S: rows k = 16*i + g, + 8
+    const float* const sin = p.state_in + ((int64_t)h * HD + col) * HD;
+#pragma unroll
+    for (int i = 0; i < kM; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            s[i][c] = p.state_in != nullptr ? sin[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] : 0.f;
+    int es[2] = {0, 0}, ex[2] = {0, 0}, ed[2] = {0, 0};
+
+    fetch(0);
+    for (int ch = 0; ch < chunks; ++ch) {
+        cp_async_wait<0>();
+        __syncthreads();  // chunk ch is there for all, and nobody still reads the other buffer
+        if (ch + 1 < chunks) fetch(ch + 1);
+        const Stage& z = st[ch & 1];
+        const bool force = (ch & 15) == 0;
+
+        uint32_t sh[kM][2], sl[kM][2];
+        gdn_col_exp(s, es, force);
+        gdn_operand(s, es, sh, sl);
+        const float su[2] = {gdn_exp2i(es[0]), gdn_exp2i(es[1])};
+        float x[4][4], o[4][4];
+        const int arow = lane & 15, acol = (lane >> 4) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float kh[4] = {}, kl[4] = {}, qh[4] = {}, ql[4] = {};
+#pragma unroll
+            for (int ks = 0; ks < kM; ++ks) {
+                uint32_t fk[4], fq[4];
+                ldmatrix_x4(fk, z.k[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                ldmatrix_x4(fq, z.q[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                mma_f16(kh, fk, sh[ks][0], sh[ks][1]);
+                mma_f16(qh, fq, sh[ks][0], sh[ks][1]);
+                mma_f16(kl, fk, sl[ks][0], sl[ks][1]);
+                mma_f16(ql, fq, sl[ks][0], sl[ks][1]);
+                if constexpr (kSplit) {
+                    ldmatrix_x4(fk, z.k[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                    ldmatrix_x4(fq, z.q[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                    mma_f16(kl, fk, sh[ks][0], sh[ks][1]);
+                    mma_f16(ql, fq, sh[ks][0], sh[ks][1]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = 16 * i + g + (c >> 1) * 8;
+                const float v = (float)z.v[r * kVLd + warp * 8 + 2 * t4 + (c & 1)];
+                x[i][c] = v - z.d.a[r] * su[c & 1] * fmaf(kl[c], 1.f / kGdnLo, kh[c]);
+                o[i][c] = z.d.b[r] * su[c & 1] * fmaf(ql[c], 1.f / kGdnLo, qh[c]);
+            }
+        }
+        // d = T X
+        uint32_t xh[4][2], xl[4][2];
+        gdn_col_exp(x, ex, force);
+        gdn_operand(x, ex, xh, xl);
+        const float xu[2] = {gdn_exp2i(ex[0]) * z.d.t_up, gdn_exp2i(ex[1]) * z.d.t_up};
+        float d[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float dh[4] = {}, dl[4] = {};
+#pragma unroll
+            for (int j = 0; j <= i; ++j) {
+                const uint4 th = z.d.t_hi[i * (i + 1) / 2 + j][lane], tl = z.d.t_lo[i * (i + 1) / 2 + j][lane];
+                mma_f16(dh, th, xh[j][0], xh[j][1]);
+                mma_f16(dl, th, xl[j][0], xl[j][1]);
+                mma_f16(dl, tl, xh[j][0], xh[j][1]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) d[i][c] = xu[c & 1] * fmaf(dl[c], 1.f / kGdnLo, dh[c]);
+        }
+        // o += P d
+        uint32_t dh[4][2], dl[4][2];
+        gdn_col_exp(d, ed, force);
+        gdn_operand(d, ed, dh, dl);
+        const float du[2] = {gdn_exp2i(ed[0]), gdn_exp2i(ed[1])};
+        const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float oh[4] = {}, ol[4] = {};
+#pragma unroll
+            for (int j = 0; j <= i; ++j) {
+                const uint4 ph = z.d.p[i * (i + 1) / 2 + j][lane];
+                mma_f16(oh, ph, dh[j][0], dh[j][1]);
+                mma_f16(ol, ph, dl[j][0], dl[j][1]);
+                if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dh[j][0], dh[j][1]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                o[i][c] = fmaf(z.d.p_up * du[c & 1], fmaf(ol[c], 1.f / kGdnLo, oh[c]), o[i][c]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int64_t t = tok0 + 16 * i + g + 8 * b;
+                if (t < p.t1) {
+                    T* const dst = static_cast<T*>(a.o) + t * a.o_row + h * HD + col;
+                    if constexpr (kSplit)
+                        *reinterpret_cast<float2*>(dst) = make_float2(o[i][2 * b], o[i][2 * b + 1]);
+                    else
+                        *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(o[i][2 * b], o[i][2 * b + 1]);
+                }
+            }
+        }
+        // S <- e^G S + K^T (c d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) d[i][c] *= z.d.c[16 * i + g + (c >> 1) * 8];
+        gdn_col_exp(d, ed, force);
+        gdn_operand(d, ed, dh, dl);
+        const float cu[2] = {gdn_exp2i(ed[0]), gdn_exp2i(ed[1])};
+        const int krow = (lane & 7) + ((lane >> 4) << 3), kcol = ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < kM; ++i) {
+            float nh[4] = {}, nl[4] = {};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t fk[4];
+                ldmatrix_x4_t(fk, z.k[0] + (j * 16 + krow) * kLd + i * 16 + kcol);
+                mma_f16(nh, fk, dh[j][0], dh[j][1]);
+                mma_f16(nl, fk, dl[j][0], dl[j][1]);
+                if constexpr (kSplit) {
+                    ldmatrix_x4_t(fk, z.k[kSplit] + (j * 16 + krow) * kLd + i * 16 + kcol);
+                    mma_f16(nl, fk, dh[j][0], dh[j][1]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                s[i][c] = fmaf(z.d.decay, s[i][c], cu[c & 1] * fmaf(nl[c], 1.f / kGdnLo, nh[c]));
+        }
+    }
+    float* const sout = a.state_out + ((int64_t)h * HD + col) * HD;
+#pragma unroll
+    for (int i = 0; i < kM; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sout[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] = s[i][c];
+}
+
+// Tokens per segment: what the prep kernel writes for a segment is still in L2 when the scan reads it.
+constexpr int64_t kGdnSegBytes = int64_t(64) << 20;
+static int64_t gdn_chunk_bytes(bool f32, int k_heads, int v_heads, int head_dim) {
+    return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * (int64_t)(4 * 64 * head_dim * 2)
+               : v_heads * (int64_t)sizeof(GdnChunkData<false>);
+}
+static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
+    const int64_t n = kGdnSegBytes / gdn_chunk_bytes(f32, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
+    return n < 1 ? 1 : (n < all ? n : all);
+}
+// Calls of at least this many tokens take the chunked form.
+constexpr int64_t kGdnChunkedFrom = 64;
+
+template <typename T, int HD>
+static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t stream) {
+    constexpr bool kSplit = sizeof(T) == 4;
+    const int64_t seg = gdn_seg_chunks(kSplit, a.T, a.k_heads, a.v_heads, HD);
+    const auto prep = gdn_chunk_prep_kernel<T, HD>;
+    const auto scan = gdn_chunk_scan_kernel<T, HD>;
+    const int prep_smem = (int)sizeof(GdnPrepSmem<T, HD>), scan_smem = (int)(2 * sizeof(GdnScanStage<T, HD>));
+    int rc = ensure_smem((const void*)prep, prep_smem);
+    if (rc == WZYB_OK) rc = ensure_smem((const void*)scan, scan_smem);
+    if (rc != WZYB_OK) return rc;
+    GdnPrepArgs pa;
+    GdnScanArgs sa;
+    pa.x = sa.x = a;
+    pa.data = ws;
+    pa.kq = reinterpret_cast<__half*>(ws + seg * a.v_heads * (int64_t)sizeof(GdnChunkData<kSplit>));
+    sa.data = pa.data;
+    sa.kq = pa.kq;
+    sa.state_in = a.state_in;
+    for (int64_t t0 = 0; t0 < a.T; t0 += seg * kGdnChunk) {
+        const int64_t t1 = t0 + seg * kGdnChunk < a.T ? t0 + seg * kGdnChunk : a.T;
+        pa.t0 = sa.t0 = t0;
+        sa.t1 = t1;
+        const int64_t chunks = (t1 - t0 + kGdnChunk - 1) / kGdnChunk;
+        launch_k(prep, (unsigned)(chunks * a.k_heads), 128, prep_smem, stream, pa);
+        launch_k(scan, a.v_heads * (HD / 32), 128, scan_smem, stream, sa);
+        sa.state_in = a.state_out;
+    }
+    return launch_status();
+}
+
 template <typename T>
 static int gdn_delta_entry(const wzyb_gdn_delta_args* p, int64_t T_, cudaStream_t stream) {
     if (p == nullptr) return WZYB_ERR_NULL;
@@ -228,6 +877,13 @@ static int gdn_delta_entry(const wzyb_gdn_delta_args* p, int64_t T_, cudaStream_
     a.scale = x.scale;
     a.l2norm = x.qk_l2norm;
     a.l2_eps = x.l2_eps;
+    if (T_ >= kGdnChunkedFrom && x.state_snaps == nullptr) {
+        if (!x.workspace) return WZYB_ERR_NULL;
+        if (!aligned16(x.workspace)) return WZYB_ERR_ALIGN;
+        if (x.workspace_bytes < wzyb_gdn_delta_rule_workspace(T_, x.k_heads, x.v_heads, x.head_dim)) return WZYB_ERR_SHAPE;
+        uint8_t* const ws = static_cast<uint8_t*>(x.workspace);
+        return x.head_dim == 64 ? launch_gdn_chunked<T, 64>(a, ws, stream) : launch_gdn_chunked<T, 128>(a, ws, stream);
+    }
     const int grid = x.v_heads * (x.head_dim / 32);
     if (x.head_dim == 64)
         launch_k(gdn_recurrent_kernel<T, 64>, grid, 256, 0, stream, a);
@@ -241,8 +897,14 @@ static int gdn_delta_entry(const wzyb_gdn_delta_args* p, int64_t T_, cudaStream_
 extern "C" {
 
 int64_t wzyb_gdn_delta_rule_workspace(int64_t T, int k_heads, int v_heads, int head_dim) {
-    (void)T, (void)k_heads, (void)v_heads, (void)head_dim;
-    return 0;
+    if (T < wzyb::kGdnChunkedFrom || k_heads < 1 || v_heads < 1 || head_dim < 1) return 0;
+    int64_t most = 0;
+    for (int f32 = 0; f32 < 2; ++f32) {
+        const int64_t bytes = wzyb::gdn_seg_chunks(f32 != 0, T, k_heads, v_heads, head_dim) *
+                              wzyb::gdn_chunk_bytes(f32 != 0, k_heads, v_heads, head_dim);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 int wzyb_gdn_delta_rule_f16(const wzyb_gdn_delta_args* a, int64_t T, wzyb_stream_t stream) {
     return wzyb::gdn_delta_entry<__half>(a, T, (cudaStream_t)stream);
