@@ -575,321 +575,526 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 }
 
 // ----------------------------------------------------------------------------------------------------
-// Many query rows per kv head (prefill, large trees): a CTA takes 16 rows per warp and walks its share of
-// 64-key tiles. The tile's codes come by cp.async as bytes while the tile before is worked through, are
-// widened once to fp16 in shared memory and used by every warp. Rows lead (x = q K^T, o = p V), so the
-// weights go from the first product's accumulators to the second's operand within each lane.
+// Many query rows per kv head (prefill, verify windows, trees): a CTA takes 128 rows and walks its share of
+// 64-key tiles on the 5th-generation tensor cores. Tensor memory (512 columns, one row per lane): columns
+// 0..255 hold a tile's scores, 64 per 64-element group (the groups' scales differ per key, so each group's
+// products have their own accumulator), and then, in the same columns, the weights: per group the fp16 copy of
+// p * vs (and for fp32 calls its second part); columns 256..511 hold the tile's p V.
+//   warps 0-7   a row is two lanes (keys 0-31 and 32-63 of the tile): scores from tensor memory, running
+//               maximum, exponentials, weights back to tensor memory; the previous tile's p V from tensor
+//               memory onto the row's o in fp32 registers (half of the head dimension each)
+//   warps 8-11  cells: the tile's codes from global memory (a tile ahead, in registers), widened to fp16 into
+//               128-byte rows of shared memory with the 128-byte swizzle. Keys and values have the same layout:
+//               K is read with the dimension contracted (K-major), V with the keys contracted (MN-major)
+//   warp 12     one lane issues the MMAs: S_g = Q_g K_g^T, then o_g = P_g V_g with P_g from tensor memory
+// o is summed in registers, not in tensor memory: the tensor cores cut their sums off towards zero, and over a
+// long context that would be a drift; it also leaves nothing to rescale there when the maximum moves.
+// Every wait is bounded: a wait that gives up sets a flag that ends all the others, and the CTA returns.
 // ----------------------------------------------------------------------------------------------------
-template <typename T, int HD, int kWarps>
-struct TileSmem {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// d = a * b + d * 2^-11
+__device__ __forceinline__ void tc_mma_ts_down11(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %4, %4, %4}, p, 11;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void tc_ld16(float (&r)[16], uint32_t at) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(at));
+}
+__device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&u)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(u[0]), "r"(u[1]),
+                 "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
+}
+// Operand descriptor of rows of 128 bytes with the 128-byte swizzle, 8-row blocks 1024 bytes apart (both as the
+// rows of a K-major operand and as the contracted index of an MN-major one of 64 columns).
+__device__ __forceinline__ uint64_t tc_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// fp16 x fp16 -> fp32, M = 128, N = 64
+constexpr uint32_t kTcIdesc = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kTcIdescBMn = kTcIdesc | (1u << 16);  // B is MN-major
+
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 0u) {
+            if (*quit) return false;
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+                raise_fault(WZYB_FAULT_WAIT_TIMEOUT);
+                *quit = 1;
+                return false;
+            }
+        }
+    }
+}
+
+template <typename T, int HD>
+struct TcSmem {
     static constexpr bool kSplit = sizeof(T) == 4;
-    static constexpr int kRows = 16 * kWarps, kLd = HD + 8, kN = 64, NG = HD / 64;
-    __half qs[kRows * kLd];
-    __half ql[kSplit ? kRows * kLd : 8];
-    __half kf[kN * kLd];
-    __half vf[kN * kLd];
-    int8_t raw[2][kN * HD];
-    float ks[kN][NG], vs[kN][NG];
+    static constexpr int kRows = 128, kN = 64, NG = HD / 64;
+    // [group][row][64 dims], 128-byte rows, swizzled
+    __half q[kSplit ? 2 : 1][NG][kRows * 64];
+    __half k[NG][kN * 64];
+    __half v[NG][kN * 64];
+    float ks[2][NG][kN], vs[2][NG][kN];
     float row_scale[kRows];
+    float x_max[2][2][kRows];  // [tile parity][half][row]
+    int x_exp[2][2][kRows];
+    int e_key[2][kN], e_max[2][2];
+    uint64_t k_full, v_full, scales, s_full[NG], p_full[NG], x_full, o_full, done;
     KeyPlan plan;
-    int e_key[kN], e_max[kWarps];
+    uint32_t tmem;
+    int quit;
 };
 
-template <typename T, int HD, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
+constexpr int kTcThreads = 512;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
     pdl_begin();
-    using S = TileSmem<T, HD, kWarps>;
+    using S = TcSmem<T, HD>;
     constexpr bool kSplit = S::kSplit;
-    constexpr int NG = S::NG, kN = S::kN, kLd = S::kLd, kThreads = kWarps * 32;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    constexpr int NG = S::NG, kN = S::kN, kHalf = HD / 2;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     S& sm = *reinterpret_cast<S*>(smem_raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const int split = blockIdx.x, row0 = blockIdx.y * S::kRows, head = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int split = blockIdx.x, row0 = (gridDim.y - 1 - blockIdx.y) * S::kRows, head = blockIdx.z;
     const int rows = a.T * a.G;
     const int64_t base = (a.d_base_pos ? (int64_t)__ldg(a.d_base_pos) : 0) + a.pos_offset;
-    if (warp == 0)
+
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (warp == 13) {
         build_plan<kN>(a, sm.plan, base, row0 / a.G, (min(row0 + S::kRows, rows) - 1) / a.G + 1, lane);
-    stage_rows<T, HD, kSplit>(a, head, row0, rows, S::kRows, sm.qs, sm.ql, kLd, sm.row_scale, warp, kWarps, lane);
+    } else if (warp == 14 && lane == 0) {
+        sm.quit = 0;
+        mbar_init(&sm.k_full, 128);
+        mbar_init(&sm.v_full, 128);
+        for (int g = 0; g < NG; ++g) {
+            mbar_init(&sm.s_full[g], 1);
+            mbar_init(&sm.p_full[g], 256);
+        }
+        mbar_init(&sm.scales, 1);
+        mbar_init(&sm.x_full, 256);
+        mbar_init(&sm.o_full, 1);
+        mbar_init(&sm.done, 1);
+        fence_mbar_init();
+    }
+    if (warp < 12) {  // query rows to shared memory, one warp per row in turn
+        constexpr int kE = HD / 32;
+        for (int r = warp; r < S::kRows; r += 12) {
+            float x[kE];
+            const int row = row0 + r;
+            if (row < rows) {
+                const int t = row / a.G, gq = row - t * a.G;
+                const T* p = static_cast<const T*>(a.q) + t * a.q_row + (int64_t)(head * a.G + gq) * a.q_head + lane * kE;
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[i] = (float)p[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[i] = 0.f;
+            }
+            float f = a.scale_log2;
+            if constexpr (kSplit) {
+                float am = 0.f;
+#pragma unroll
+                for (int i = 0; i < kE; ++i) am = fmaxf(am, fabsf(x[i]));
+                am = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
+                int e = scale_exp(am);
+                if (e < -100 || e > 120) e = 0;
+                const float down = exp2_int(-e);
+                f *= exp2_int(e);
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[i] *= down;
+            }
+            const int g = lane * kE / 64, c = (lane * kE % 64) * 2;  // byte in the 128-byte row
+            const int at = r * 128 + ((((c >> 4) ^ (r & 7)) << 4) | (c & 15));
+            uint32_t h[kE / 2], l[kE / 2];
+#pragma unroll
+            for (int i = 0; i < kE / 2; ++i) {
+                h[i] = pack_f16(x[2 * i], x[2 * i + 1]);
+                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+                l[i] = pack_f16(x[2 * i] - y.x, x[2 * i + 1] - y.y);
+            }
+#pragma unroll
+            for (int i = 0; i < kE / 2; ++i) {
+                *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at + 4 * i) = h[i];
+                if constexpr (kSplit) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sm.q[kSplit][g]) + at + 4 * i) = l[i];
+            }
+            if (lane == 0) sm.row_scale[r] = f;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
     const KeyPlan& plan = sm.plan;
     const int ntiles = plan.first[plan.ranges];
     const int tb = (int)((int64_t)ntiles * split / a.splits), te = (int)((int64_t)ntiles * (split + 1) / a.splits);
-    const int kvd = a.kv_heads * HD, spc = a.kv_heads * NG;
+    const uint32_t tmem = sm.tmem;
+    volatile int* const quit = &sm.quit;
 
-    int rt[2];
-    RowSpan span[2];
-    float rs[2];
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int half = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + r;
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
+        const int t = min(row, rows - 1) / a.G;
+        const RowSpan span = row_span(a, base, t);
+        const float rs = sm.row_scale[r];
+        float o[kHalf];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        rt[i] = min(row0 + warp * 16 + g + 8 * i, rows - 1) / a.G;
-        span[i] = row_span(a, base, rt[i]);
-        rs[i] = sm.row_scale[warp * 16 + g + 8 * i];
-    }
-
-    // bytes of tile `it` into sm.raw; keys past the tile's end are not fetched (their bytes are whatever
-    // the buffer held: finite codes, whose scales count as 0)
-    auto fetch = [&](int it) {
-        const KeyTile kt = key_tile<kN>(plan, it);
-        const Planes pl = planes_of<HD>(a, kt.draft, head);
-        constexpr int kChunks = HD / 16;
-#pragma unroll 4
-        for (int i = tid; i < kN * kChunks; i += kThreads) {
-            const int key = i / kChunks, c = (i % kChunks) * 16;
-            if (key >= kt.count) continue;
-            const int64_t at = cell_of(a, kt.draft, kt.pos + key) * kvd + c;
-            cp_async16(&sm.raw[0][key * HD + c], pl.kq + at);
-            cp_async16(&sm.raw[1][key * HD + c], pl.vq + at);
-        }
-        cp_async_commit();
-    };
-    // scales of one key per thread
-    float nks[NG], nvs[NG];
-    auto fetch_scales = [&](int it) {
+        for (int i = 0; i < kHalf; ++i) o[i] = 0.f;
+        float m = -INFINITY, l = 0.f, alpha = 1.f;
+        int E = -1000;
+        auto unit = [](int e) { return e <= -1000 ? 7 : e; };  // while only scales of 0 have been seen
+        bool ok = true;
+        // the previous tile's p V onto o
+        auto drain = [&](uint32_t parity) {
+            ok = __all_sync(0xffffffffu, tc_wait(&sm.o_full, parity, quit));
+            if (!ok) return;
+            tc_fence_after();
 #pragma unroll
-        for (int n = 0; n < NG; ++n) nks[n] = nvs[n] = 0.f;
-        if (tid < kN) {
+            for (int c = 0; c < kHalf; c += 16) {
+                float x[16];
+                tc_ld16(x, mine + 256 + half * kHalf + c);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 y = ffma2(make_float2(o[c + i], o[c + i + 1]), splat2(alpha), make_float2(x[i], x[i + 1]));
+                    o[c + i] = y.x;
+                    o[c + i + 1] = y.y;
+                }
+            }
+        };
+        for (int it = tb; it < te && ok; ++it) {
+            const int n = it - tb, b = n & 1;
+            if (n > 0) {
+                drain((n - 1) & 1);
+                if (!ok) break;
+            }
+            ok = __all_sync(0xffffffffu, tc_wait(&sm.scales, b, quit));
+            if (!ok) break;
+            float s[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                ok = ok && __all_sync(0xffffffffu, tc_wait(&sm.s_full[g], b, quit));
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 32; c += 16) {
+                    float x[16];
+                    tc_ld16(x, mine + g * 64 + half * 32 + c);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&sm.ks[b][g][half * 32 + c + i]);
+                        const float2 y0 = ffma2(make_float2(x[i], x[i + 1]), make_float2(f.x, f.y), make_float2(s[c + i], s[c + i + 1]));
+                        const float2 y1 = ffma2(make_float2(x[i + 2], x[i + 3]), make_float2(f.z, f.w), make_float2(s[c + i + 2], s[c + i + 3]));
+                        s[c + i] = y0.x;
+                        s[c + i + 1] = y0.y;
+                        s[c + i + 2] = y1.x;
+                        s[c + i + 3] = y1.y;
+                    }
+                }
+            }
+            if (!ok) break;
             const KeyTile kt = key_tile<kN>(plan, it);
-            if (tid < kt.count) {
-                const Planes pl = planes_of<HD>(a, kt.draft, head);
-                const int64_t at = cell_of(a, kt.draft, kt.pos + tid) * spc;
-                load_scales<NG>(pl.ks + at, nks);
-                load_scales<NG>(pl.vs + at, nvs);
-            }
-        }
-    };
-
-    float o[HD / 8][4];
+            const bool masked = !tile_unmasked<kN>(plan, kt);  // CTA-uniform
+            float top = -INFINITY;
+            int e = max(sm.e_max[b][0], sm.e_max[b][1]);
+            if (!masked) {
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
+                for (int i = 0; i < 32; ++i) {
+                    s[i] *= rs;
+                    top = fmaxf(top, s[i]);
+                }
+            } else {
+                uint32_t see = 0;
+                const int key0 = half * 32;
+                if (kt.draft) {
+                    const int wd = (kt.pos + key0) >> 5;
+                    if (wd < a.mask_words) see = __ldg(a.mask + (int64_t)t * a.mask_words + wd);
+                    if (kt.count < key0 + 32) see &= kt.count > key0 ? (1u << (kt.count - key0)) - 1u : 0u;
+                } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int E[2] = {-1000, -1000};
-    for (int i = tid; i < (int)sizeof(sm.raw) / 16; i += kThreads) reinterpret_cast<uint4*>(sm.raw)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-
-    if (tb < te) {
-        fetch(tb);
-        fetch_scales(tb);
-    }
-    for (int it = tb; it < te; ++it) {
-        cp_async_wait<0>();
-        int e = -1000;
-        if (tid < kN) {
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                sm.ks[tid][n] = nks[n];
-                sm.vs[tid][n] = nvs[n];
-                e = max(e, scale_exp(nvs[n]));
-            }
-            sm.e_key[tid] = e;
-        }
-        e = __reduce_max_sync(0xffffffffu, e);
-        if (lane == 0) sm.e_max[warp] = e;
-        __syncthreads();
-        for (int i = tid; i < kN * HD / 16; i += kThreads) {
-            const int key = i / (HD / 16), c = (i % (HD / 16)) * 16;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const uint4 w = *reinterpret_cast<const uint4*>(&sm.raw[b][key * HD + c]);
-                const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-                uint4* const d = reinterpret_cast<uint4*>((b ? sm.vf : sm.kf) + key * kLd + c);
-                d[0] = make_uint4(codes_f16(x[0], kSelLo), codes_f16(x[0], kSelHi), codes_f16(x[1], kSelLo),
-                                  codes_f16(x[1], kSelHi));
-                d[1] = make_uint4(codes_f16(x[2], kSelLo), codes_f16(x[2], kSelHi), codes_f16(x[3], kSelLo),
-                                  codes_f16(x[3], kSelHi));
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) e = max(e, sm.e_max[w]);
-        __syncthreads();
-        const KeyTile kt = key_tile<kN>(plan, it);
-        if (it + 1 < te) {
-            fetch(it + 1);
-            fetch_scales(it + 1);
-        }
-
-        float s[kN / 8][4];
-#pragma unroll
-        for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) s[i][c] = 0.f;
-        const int qrow = warp * 16 + (lane & 15), qcol = (lane >> 4) * 8;
-        const int krow = (lane & 7) + ((lane >> 4) << 3), kcol = ((lane >> 3) & 1) * 8;
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            float acc[kN / 8][4];
-#pragma unroll
-            for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-                uint32_t fa[4], fl[4];
-                ldmatrix_x4(fa, sm.qs + qrow * kLd + n * 64 + kk * 16 + qcol);
-                if constexpr (kSplit) ldmatrix_x4(fl, sm.ql + qrow * kLd + n * 64 + kk * 16 + qcol);
-#pragma unroll
-                for (int i = 0; i < kN / 16; ++i) {
-                    uint32_t fb[4];
-                    ldmatrix_x4(fb, sm.kf + (i * 16 + krow) * kLd + n * 64 + kk * 16 + kcol);
-                    mma_f16(acc[2 * i], fa, fb[0], fb[1]);
-                    mma_f16(acc[2 * i + 1], fa, fb[2], fb[3]);
-                    if constexpr (kSplit) {
-                        mma_f16(acc[2 * i], fl, fb[0], fb[1]);
-                        mma_f16(acc[2 * i + 1], fl, fb[2], fb[3]);
+                    for (int i = 0; i < 32; ++i) {
+                        const int pos = kt.pos + key0 + i;
+                        if (key0 + i < kt.count && pos <= span.hi && (pos < plan.sinks || pos > span.lo)) see |= 1u << i;
                     }
                 }
-            }
+                e = -1000;
 #pragma unroll
-            for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][c] = fmaf(acc[i][c], sm.ks[i * 8 + 2 * t4 + (c & 1)][n], s[i][c]);
-        }
-        float top[2] = {-INFINITY, -INFINITY};
-        int er[2] = {e, e};
-        if (tile_unmasked<kN>(plan, kt)) {  // CTA-uniform
-#pragma unroll
-            for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    s[i][c] *= rs[c >> 1];
-                    top[c >> 1] = fmaxf(top[c >> 1], s[i][c]);
-                }
-        } else {
-            er[0] = er[1] = -1000;
-#pragma unroll
-            for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    s[i][c] *= rs[c >> 1];
-                    const int key = i * 8 + 2 * t4 + (c & 1), pos = kt.pos + key;
-                    bool see = key < kt.count;
-                    if (kt.draft) {
-                        if (see) see = (__ldg(a.mask + (int64_t)rt[c >> 1] * a.mask_words + (pos >> 5)) >> (pos & 31)) & 1u;
+                for (int i = 0; i < 32; ++i) {
+                    if (see >> i & 1u) {
+                        s[i] *= rs;
+                        e = max(e, sm.e_key[b][key0 + i]);
                     } else {
-                        see = see && pos <= span[c >> 1].hi && (pos < plan.sinks || pos > span[c >> 1].lo);
+                        s[i] = -INFINITY;
                     }
-                    if (see)
-                        er[c >> 1] = max(er[c >> 1], sm.e_key[key]);
-                    else
-                        s[i][c] = -INFINITY;
-                    top[c >> 1] = fmaxf(top[c >> 1], s[i][c]);
-                }
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f || er[0] > E[0] || er[1] > E[1])) {
-            float alpha[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int x = 1; x < 4; x <<= 1) {
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], x));
-                    er[i] = max(er[i], __shfl_xor_sync(0xffffffffu, er[i], x));
-                }
-                alpha[i] = 1.f;
-                if (top[i] > m[i] + 8.f || er[i] > E[i]) {
-                    top[i] = fmaxf(top[i], m[i]);
-                    er[i] = max(er[i], E[i]);
-                    alpha[i] = ex2_approx(m[i] - (top[i] == -INFINITY ? 0.f : top[i]));
-                    l[i] *= alpha[i];
-                    alpha[i] *= exp2_int(E[i] - er[i]);
-                    m[i] = top[i];
-                    E[i] = er[i];
+                    top = fmaxf(top, s[i]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[i][c] *= alpha[c >> 1];
-        }
-        const float mr[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-        for (int i = 0; i < kN / 8; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[i][c] = ex2_approx(s[i][c] - mr[c >> 1]);
-                l[c >> 1] += s[i][c];
+            sm.x_max[b][half][r] = top;
+            sm.x_exp[b][half][r] = e;
+            mbar_arrive(&sm.x_full);
+            // also: every score has been read, so weights may take their columns
+            ok = __all_sync(0xffffffffu, tc_wait(&sm.x_full, b, quit));
+            if (!ok) break;
+            top = fmaxf(top, sm.x_max[b][half ^ 1][r]);
+            e = max(e, sm.x_exp[b][half ^ 1][r]);
+            alpha = 1.f;
+            if (top > m + 8.f || e > E) {
+                top = fmaxf(top, m);
+                e = max(e, E);
+                alpha = ex2_approx(m - (top == -INFINITY ? 0.f : top)) * exp2_int(unit(E) - unit(e));
+                l *= alpha;
+                m = top;
+                E = e;
             }
-        float up[2];
+            // p * 2^(7 - E), so that p * vs has the weights' size; l sums these
+            const float shift = (m == -INFINITY ? 0.f : m) - (float)(7 - unit(E));
+            float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) up[i] = E[i] <= -1000 ? 0.f : exp2_int(7 - E[i]);
-        const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vcol = (lane >> 4) * 8;
+            for (int i = 0; i < 32; ++i) {
+                s[i] = ex2_approx(s[i] - shift);
+                sum += s[i];
+            }
+            l += sum;
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            // the tile's products of one group, added to o afterwards: the tensor cores cut each sum off
-            // towards zero, which over thousands of tiles would be a drift of the running sums
-            float acc[8][4];
+            for (int g = 0; g < NG; ++g) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[j][c] = 0.f;
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&sm.vs[b][g][half * 32 + c + i]);
+                        float w[4] = {s[c + i] * f.x, s[c + i + 1] * f.y, s[c + i + 2] * f.z, s[c + i + 3] * f.w};
+                        if (masked) {  // a weight of 0 stays 0 whatever the cell's scale (infinite or NaN) is
 #pragma unroll
-            for (int part = kSplit ? 1 : 0; part >= 0; --part) {  // fp32 calls: the second parts first
-#pragma unroll
-                for (int kk = 0; kk < kN / 16; ++kk) {
-                    uint32_t fa[4];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {  // keys kk*16 + b*8 + 2*t4, + 1
-                        const float v0 = sm.vs[kk * 16 + b * 8 + 2 * t4][n], v1 = sm.vs[kk * 16 + b * 8 + 2 * t4 + 1][n];
-                        const float (&p)[4] = s[2 * kk + b];
-                        // masked places: a weight of 0 stays 0 whatever the cell's scale (infinite or NaN) is
-                        const float w[4] = {p[0] == 0.f ? 0.f : p[0] * (v0 * up[0]), p[1] == 0.f ? 0.f : p[1] * (v1 * up[0]),
-                                            p[2] == 0.f ? 0.f : p[2] * (v0 * up[1]), p[3] == 0.f ? 0.f : p[3] * (v1 * up[1])};
-                        if (part == 1) {
-                            uint32_t hi;
-                            split_f16(w[0], w[1], hi, fa[2 * b]);
-                            split_f16(w[2], w[3], hi, fa[2 * b + 1]);
+                            for (int j = 0; j < 4; ++j) w[j] = s[c + i + j] == 0.f ? 0.f : w[j];
+                        }
+                        if constexpr (kSplit) {
+                            split_f16(w[0], w[1], hi[i / 2], lo[i / 2]);
+                            split_f16(w[2], w[3], hi[i / 2 + 1], lo[i / 2 + 1]);
                         } else {
-                            fa[2 * b] = pack_f16(w[0], w[1]);
-                            fa[2 * b + 1] = pack_f16(w[2], w[3]);
+                            hi[i / 2] = pack_f16(w[0], w[1]);
+                            hi[i / 2 + 1] = pack_f16(w[2], w[3]);
                         }
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t fb[4];
-                        ldmatrix_x4_t(fb, sm.vf + (kk * 16 + vrow) * kLd + n * 64 + j * 16 + vcol);
-                        mma_f16(acc[2 * j], fa, fb[0], fb[1]);
-                        mma_f16(acc[2 * j + 1], fa, fb[2], fb[3]);
-                    }
+                    tc_st8(mine + g * 64 + half * 16 + c / 2, hi);
+                    if constexpr (kSplit) tc_st8(mine + g * 64 + 32 + half * 16 + c / 2, lo);
                 }
-                if (part == 1) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) acc[j][c] *= 1.f / kLoUp;
-                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.p_full[g]);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[n * 8 + j][c] += acc[j][c];
         }
-        __syncthreads();  // kf, vf and the scales are free
-    }
-
+        if (te > tb && ok) drain((te - tb - 1) & 1);
+        // the row's sum over both halves of the keys, then its o (or its part of it)
+        sm.x_max[0][half][r] = l;
+        mbar_arrive(&sm.x_full);
+        ok = ok && tc_wait(&sm.x_full, (te - tb) & 1, quit);
+        l += sm.x_max[0][half ^ 1][r];
+        if (row < rows && ok) {
+            const int gq = row - t * a.G, hq = head * a.G + gq;
+            const int64_t orow = (int64_t)t * a.G * a.kv_heads + hq;
+            const float back = exp2_int(unit(E) - 7);  // of l and of o
+            if (a.splits == 1) {
+                const float norm = l == 0.f ? 0.f : 1.f / l;
+                if (half == 0 && a.lse != nullptr)
+                    a.lse[orow] = l == 0.f ? -INFINITY : (m + (float)(unit(E) - 7) + log2f(l)) * 0.6931471805599453f;
+                T* const p = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + half * kHalf;
+                if constexpr (kSplit) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float back = E[i] <= -1000 ? 0.f : exp2_int(E[i] - 7);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int row = row0 + warp * 16 + g + 8 * i;
-        if (row >= rows) continue;
-        const int t = row / a.G, hq = head * a.G + (row - t * a.G);
-        const int64_t orow = (int64_t)t * a.G * a.kv_heads + hq;
-        if (a.splits == 1) {
-            const float norm = l[i] == 0.f ? 0.f : back / l[i];
-            if (t4 == 0 && a.lse != nullptr) a.lse[orow] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * 0.6931471805599453f;
-            T* const p = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + 2 * t4;
+                    for (int i = 0; i < kHalf; i += 4)
+                        *reinterpret_cast<float4*>(p + i) = make_float4(o[i] * norm, o[i + 1] * norm, o[i + 2] * norm, o[i + 3] * norm);
+                } else {
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) store_out2(p + n * 8, o[n][2 * i] * norm, o[n][2 * i + 1] * norm);
-        } else {
-            const int64_t at = (int64_t)split * rows * a.kv_heads + orow;
-            if (t4 == 0) a.part_ml[at] = make_float2(m[i], l[i]);
-            float* const p = a.part_o + at * HD + 2 * t4;
+                    for (int i = 0; i < kHalf; i += 8)
+                        *reinterpret_cast<uint4*>(p + i) =
+                            make_uint4(pack_f16(o[i] * norm, o[i + 1] * norm), pack_f16(o[i + 2] * norm, o[i + 3] * norm),
+                                       pack_f16(o[i + 4] * norm, o[i + 5] * norm), pack_f16(o[i + 6] * norm, o[i + 7] * norm));
+                }
+            } else {
+                const int64_t at = (int64_t)split * rows * a.kv_heads + orow;
+                if (half == 0) a.part_ml[at] = make_float2(m, l * back);
+                float* const p = a.part_o + at * HD + half * kHalf;
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-                *reinterpret_cast<float2*>(p + n * 8) = make_float2(o[n][2 * i] * back, o[n][2 * i + 1] * back);
+                for (int i = 0; i < kHalf; i += 4)
+                    *reinterpret_cast<float4*>(p + i) = make_float4(o[i] * back, o[i + 1] * back, o[i + 2] * back, o[i + 3] * back);
+            }
+        }
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        const int u = tid - 256;
+        constexpr int kCh = HD / 16, kKeys = kN * kCh / 128;  // 16-byte pieces of a row; rows per thread
+        const int c = u % kCh, key0 = u / kCh;
+        uint4 kr[kKeys], vr[kKeys];
+        float sc[NG];  // K scales of key u (u < 64) or V scales of key u - 64
+        int cells[kKeys];
+        auto find = [&](int it) {
+            const KeyTile kt = key_tile<kN>(plan, it);
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                const int key = key0 + i * (128 / kCh);
+                cells[i] = key < kt.count ? (int)cell_of(a, kt.draft, kt.pos + key) : -1;
+            }
+        };
+        const int kvd = a.kv_heads * HD, spc = a.kv_heads * NG;
+        // keys past the tile's end: zero codes and zero scales
+        auto load = [&](uint4 (&x)[kKeys], int it, bool value) {
+            const bool draft = key_tile<kN>(plan, it).draft;
+            const Planes pl = planes_of<HD>(a, draft, head);
+            const int8_t* const src = (value ? pl.vq : pl.kq) + c * 16;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+                x[i] = cells[i] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(src + (int64_t)cells[i] * kvd));
+        };
+        auto load_sc = [&](int it) {
+            const KeyTile kt = key_tile<kN>(plan, it);
+            const Planes pl = planes_of<HD>(a, kt.draft, head);
+            const int key = u & 63;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) sc[g] = 0.f;
+            if (key < kt.count) load_scales<NG>((u < 64 ? pl.ks : pl.vs) + cell_of(a, kt.draft, kt.pos + key) * spc, sc);
+        };
+        auto widen = [&](const uint4 (&x)[kKeys], __half (&dst)[NG][kN * 64]) {
+            uint8_t* const d = reinterpret_cast<uint8_t*>(dst[c / 4]);
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                const int key = key0 + i * (128 / kCh), c16 = (c % 4) * 2;
+                const uint32_t w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u};
+                *reinterpret_cast<uint4*>(d + key * 128 + ((c16 ^ (key & 7)) << 4)) =
+                    make_uint4(codes_f16(w[0], kSelLo), codes_f16(w[0], kSelHi), codes_f16(w[1], kSelLo), codes_f16(w[1], kSelHi));
+                *reinterpret_cast<uint4*>(d + key * 128 + (((c16 + 1) ^ (key & 7)) << 4)) =
+                    make_uint4(codes_f16(w[2], kSelLo), codes_f16(w[2], kSelHi), codes_f16(w[3], kSelLo), codes_f16(w[3], kSelHi));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        bool ok = true;
+        if (tb < te) {
+            find(tb);
+            load_sc(tb);
+            load(kr, tb, false);
+            load(vr, tb, true);
+        }
+        for (int it = tb; it < te; ++it) {
+            const int n = it - tb, b = n & 1;
+            if (n > 0) ok = __all_sync(0xffffffffu, tc_wait(&sm.s_full[NG - 1], b ^ 1, quit));  // K's memory is free
+            if (!ok) break;
+            int e = -1000;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                (u < 64 ? sm.ks : sm.vs)[b][g][u & 63] = sc[g];
+                e = max(e, scale_exp(sc[g]));
+            }
+            if (u >= 64) {
+                sm.e_key[b][u - 64] = e;
+                e = __reduce_max_sync(0xffffffffu, e);
+                if (lane == 0) sm.e_max[b][(u - 64) >> 5] = e;
+            }
+            widen(kr, sm.k);
+            mbar_arrive(&sm.k_full);
+            if (it + 1 < te) {
+                find(it + 1);
+                load_sc(it + 1);
+                load(kr, it + 1, false);
+            }
+            if (n > 0) ok = __all_sync(0xffffffffu, tc_wait(&sm.o_full, b ^ 1, quit));  // V's memory is free
+            if (!ok) break;
+            widen(vr, sm.v);
+            mbar_arrive(&sm.v_full);
+            if (it + 1 < te) load(vr, it + 1, true);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == 12 && lane == 0 && tb < te) {
+            const uint64_t qd = tc_desc(smem_u32(sm.q[0][0])), ql = tc_desc(smem_u32(sm.q[kSplit ? 1 : 0][0]));
+            const uint64_t kd = tc_desc(smem_u32(sm.k[0])), vd = tc_desc(smem_u32(sm.v[0]));
+            constexpr uint64_t kQG = S::kRows * 128 >> 4, kKG = kN * 128 >> 4;  // a group's bytes in descriptor units
+            bool ok = true;
+            for (int n = 0; n < te - tb && ok; ++n) {
+                const int b = n & 1;
+                if (n > 0) ok = tc_wait(&sm.o_full, b ^ 1, quit);  // the weights' columns are free
+                ok = ok && tc_wait(&sm.k_full, b, quit);
+                if (!ok) break;
+                mbar_arrive(&sm.scales);  // hands the cell warps' scales on to the softmax warps
+                tc_fence_after();
+#pragma unroll 1
+                for (int g = 0; g < NG; ++g) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        tc_mma_ss(tmem + g * 64, qd + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, x > 0);
+                    if constexpr (kSplit) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            tc_mma_ss(tmem + g * 64, ql + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, 1);
+                    }
+                    tc_commit(&sm.s_full[g]);
+                }
+                ok = tc_wait(&sm.v_full, b, quit);
+#pragma unroll 1
+                for (int g = 0; g < NG; ++g) {
+                    ok = ok && tc_wait(&sm.p_full[g], b, quit);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + 256 + g * 64, p = tmem + g * 64;
+                    if constexpr (kSplit) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            tc_mma_ts(d, p + 32 + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, x > 0);
+                        tc_mma_ts_down11(d, p, vd + g * kKG, kTcIdescBMn);
+                    } else {
+                        tc_mma_ts(d, p, vd + g * kKG, kTcIdescBMn, 0);
+                    }
+#pragma unroll
+                    for (int x = 1; x < 4; ++x) tc_mma_ts(d, p + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, 1);
+                }
+                if (!ok) break;
+                tc_commit(&sm.o_full);
+            }
+            // nothing of this CTA's is in flight when its memory goes
+            tc_commit(&sm.done);
+            mbar_wait_until(&sm.done, 0, globaltimer_ns() + kWaitLimitNs);
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // Joins the splits' parts of one row per CTA, in split order: HD / 4 lanes of 4 elements, the other threads
@@ -957,19 +1162,19 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
 
 // Which kernel a call takes and how far the keys may be split, from the sizes alone (the key count is only
 // known on the device). The workspace function and the launcher share it.
-constexpr int kAttnCtas = 296;  // two CTAs per SM
+constexpr int kAttnSms = 148;  // two CTAs per SM for few rows, one for many
 struct AttnShape {
     bool few;
     int tile_rows, row_tiles, max_splits;
 };
-static AttnShape attn_shape(int64_t T, int q_heads, int kv_heads, bool f32) {
+static AttnShape attn_shape(int64_t T, int q_heads, int kv_heads) {
     AttnShape s;
     const int64_t rows = T * (q_heads / kv_heads);
     s.few = rows <= 16;
-    s.tile_rows = s.few ? 8 : (f32 || rows <= 64 ? 64 : 128);
+    s.tile_rows = s.few ? 8 : 128;
     s.row_tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
-    const int64_t ctas = (int64_t)s.row_tiles * kv_heads;
-    s.max_splits = (int)(ctas >= (s.few ? kAttnCtas : kAttnCtas / 2) ? 1 : (s.few ? kAttnCtas : kAttnCtas / 2) / ctas);
+    const int64_t ctas = (int64_t)s.row_tiles * kv_heads, most = s.few ? 2 * kAttnSms : kAttnSms;
+    s.max_splits = (int)(ctas >= most ? 1 : most / ctas);
     return s;
 }
 
@@ -979,16 +1184,12 @@ static int launch_attn(KvAttnArgs& a, const AttnShape& s, cudaStream_t stream) {
     int rc = WZYB_OK;
     if (s.few) {
         launch_k(kv_attn_few_kernel<T, HD>, grid, 128, 0, stream, a);
-    } else if (s.tile_rows == 64) {
-        const auto kern = kv_attn_tile_kernel<T, HD, 4>;
-        rc = ensure_smem((const void*)kern, (int)sizeof(TileSmem<T, HD, 4>));
+    } else {
+        const auto kern = kv_attn_tile_kernel<T, HD>;
+        const int smem = (int)sizeof(TcSmem<T, HD>);
+        rc = ensure_smem((const void*)kern, smem);
         if (rc != WZYB_OK) return rc;
-        launch_k(kern, grid, 128, sizeof(TileSmem<T, HD, 4>), stream, a);
-    } else if constexpr (sizeof(T) == 2) {
-        const auto kern = kv_attn_tile_kernel<T, HD, 8>;
-        rc = ensure_smem((const void*)kern, (int)sizeof(TileSmem<T, HD, 8>));
-        if (rc != WZYB_OK) return rc;
-        launch_k(kern, grid, 256, sizeof(TileSmem<T, HD, 8>), stream, a);
+        launch_k(kern, grid, kTcThreads, smem, stream, a);
     }
     if (a.splits > 1) launch_k(kv_attn_join_kernel<T, HD>, a.T * a.G * a.kv_heads, 256, 0, stream, a);
     return launch_status();
@@ -1031,7 +1232,7 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
         ((uintptr_t)depth & 3) != 0)
         return WZYB_ERR_ALIGN;
     if (T_ == 0) return WZYB_OK;
-    const AttnShape s = attn_shape(T_, x.q_heads, x.kv_heads, sizeof(T) == 4);
+    const AttnShape s = attn_shape(T_, x.q_heads, x.kv_heads);
     if (s.max_splits > 1) {
         if (!x.workspace) return WZYB_ERR_NULL;
         if (!aligned16(x.workspace)) return WZYB_ERR_ALIGN;
@@ -1089,13 +1290,8 @@ extern "C" {
 
 int64_t wzyb_kv_attn_workspace(int64_t T, int q_heads, int kv_heads, int head_dim) {
     if (T < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 || head_dim < 1) return 0;
-    int64_t most = 0;
-    for (int f32 = 0; f32 < 2; ++f32) {
-        const int64_t n = wzyb::attn_shape(T, q_heads, kv_heads, f32 != 0).max_splits;
-        const int64_t bytes = n > 1 ? n * T * q_heads * (head_dim * 4 + 8) + 16 : 0;
-        most = bytes > most ? bytes : most;
-    }
-    return most;
+    const int64_t n = wzyb::attn_shape(T, q_heads, kv_heads).max_splits;
+    return n > 1 ? n * T * q_heads * (head_dim * 4 + 8) + 16 : 0;
 }
 int wzyb_kv_attn_f16(const wzyb_kv_attn_args* a, int64_t T, wzyb_stream_t stream) {
     return wzyb::attn_entry<__half>(a, nullptr, nullptr, nullptr, false, T, (cudaStream_t)stream);
