@@ -16,6 +16,8 @@
 // row's running maximum moves only when a score passes it by 2^8: its weights stay below 2^15 either way.
 // The second part of an fp32 call's weight enters 2^11 times as large and its products come back by 2^-11,
 // so that it is not cut off at fp16's smallest number.
+#include <type_traits>
+
 #include "launch.hpp"
 #include "common.cuh"
 
@@ -182,25 +184,29 @@ __device__ __forceinline__ Planes planes_of(const KvAttnArgs& a, bool draft, int
     return p;
 }
 
-// HD / 64 consecutive fp16 scales (aligned to their own size) as fp32.
+// HD / 64 consecutive fp16 scales (aligned to their own size)
 template <int NG>
-__device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[NG]) {
+__device__ __forceinline__ void load_scale_bits(const uint16_t* p, uint16_t (&s)[NG]) {
     if constexpr (NG == 4) {
         const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-        s[0] = x.x;
-        s[1] = x.y;
-        s[2] = y.x;
-        s[3] = y.y;
+        s[0] = (uint16_t)u.x;
+        s[1] = (uint16_t)(u.x >> 16);
+        s[2] = (uint16_t)u.y;
+        s[3] = (uint16_t)(u.y >> 16);
     } else if constexpr (NG == 2) {
         const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(p));
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u));
-        s[0] = x.x;
-        s[1] = x.y;
+        s[0] = (uint16_t)u;
+        s[1] = (uint16_t)(u >> 16);
     } else {
-        s[0] = __half2float(__ushort_as_half(__ldg(p)));
+        s[0] = __ldg(p);
     }
+}
+template <int NG>
+__device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[NG]) {
+    uint16_t u[NG];
+    load_scale_bits<NG>(p, u);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) s[g] = __half2float(__ushort_as_half(u[g]));
 }
 
 // Two int8 codes as fp16, exactly: with the sign bit flipped (u = c + 128) the byte under the high byte
@@ -216,9 +222,10 @@ constexpr uint32_t kSelLo = 0x4140u, kSelHi = 0x4342u;  // bytes 0, 1 and bytes 
 constexpr float kLoUp = 2048.f;
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack_f16((x - f.x) * kLoUp, (y - f.y) * kLoUp);
+    // 2^11 (x - h), exact: the difference and both products by powers of two are
+    const float2 r = ffma2(__half22float2(h), splat2(-kLoUp), fmul2(make_float2(x, y), splat2(kLoUp)));
+    lo = pack_f16(r.x, r.y);
 }
 
 // Exponent e with x < 2^e <= 2x for a positive finite scale, -1000 for 0, infinities and NaN: the running
@@ -580,48 +587,54 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 // 0..255 hold a tile's scores, 64 per 64-element group (the groups' scales differ per key, so each group's
 // products have their own accumulator), and then, in the same columns, the weights: per group the fp16 copy of
 // p * vs (and for fp32 calls its second part); columns 256..511 hold the tile's p V.
-//   warps 0-7   a row is two lanes (keys 0-31 and 32-63 of the tile): scores from tensor memory, running
-//               maximum, exponentials, weights back to tensor memory; the previous tile's p V from tensor
-//               memory onto the row's o in fp32 registers (half of the head dimension each)
-//   warps 8-11  cells: the tile's codes from global memory (a tile ahead, in registers), widened to fp16 into
+//   softmax warps (8 for fp32 calls, 16 for fp16): a row is 2 or 4 lanes, each with a share of the tile's keys:
+//               scores from tensor memory, running maximum, exponentials, weights back to tensor memory
+//   cell warps (4): the tile's codes from global memory (K a tile ahead, V a product ahead, in registers), widened to fp16 into
 //               128-byte rows of shared memory with the 128-byte swizzle. Keys and values have the same layout:
 //               K is read with the dimension contracted (K-major), V with the keys contracted (MN-major)
-//   warp 12     one lane issues the MMAs: S_g = Q_g K_g^T, then o_g = P_g V_g with P_g from tensor memory
-// o is summed in registers, not in tensor memory: the tensor cores cut their sums off towards zero, and over a
-// long context that would be a drift; it also leaves nothing to rescale there when the maximum moves.
-// Every wait is bounded: a wait that gives up sets a flag that ends all the others, and the CTA returns.
+//   one warp    issues the MMAs: S_g = Q_g K_g^T, then o_g = P_g V_g with P_g from tensor memory
+// fp16 calls sum o in tensor memory and scale it there when a row's maximum moves. The tensor cores cut their
+// sums off towards zero, which is a drift of about 2^-25 per 16 keys: fine for an fp16 result, not for an fp32
+// one. fp32 calls take every tile's p V from tensor memory onto fp32 registers instead (64 to 128 a lane,
+// which is why they have 8 softmax warps).
+// Every wait is bounded.
 // ----------------------------------------------------------------------------------------------------
+// Issued by one elected lane of a converged warp: the warp-uniform operands stay in uniform registers (inside an
+// `if (lane == 0)` each MMA cost about 130 cycles of moving them there, 4 times its own time).
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(add)
         : "memory");
 }
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(add)
         : "memory");
 }
 // d = a * b + d * 2^-11
 __device__ __forceinline__ void tc_mma_ts_down11(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %4, %4, %4}, p, 11;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, 1, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %4, %4, %4}, p, 11;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(0)
         : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 16 columns of this warp's 32 lanes
-__device__ __forceinline__ void tc_ld16(float (&r)[16], uint32_t at) {
+__device__ __forceinline__ void tc_ld16(float* r, uint32_t at) {
     uint32_t* u = reinterpret_cast<uint32_t*>(r);
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -629,10 +642,22 @@ __device__ __forceinline__ void tc_ld16(float (&r)[16], uint32_t at) {
           "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
         : "r"(at));
 }
-__device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&u)[8]) {
+__device__ __forceinline__ void tc_st(uint32_t at, const uint32_t (&u)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st(uint32_t at, const uint32_t (&u)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(u[0]), "r"(u[1]),
                  "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                  : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t at, const float (&r)[16]) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+        : "memory");
 }
 // Operand descriptor of rows of 128 bytes with the 128-byte swizzle, 8-row blocks 1024 bytes apart (both as the
 // rows of a K-major operand and as the contracted index of an MN-major one of 64 columns).
@@ -644,117 +669,143 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t smem_addr) {
 constexpr uint32_t kTcIdesc = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kTcIdescBMn = kTcIdesc | (1u << 16);  // B is MN-major
 
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = globaltimer_ns();
-    for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 0u) {
-            if (*quit) return false;
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
-                raise_fault(WZYB_FAULT_WAIT_TIMEOUT);
-                *quit = 1;
-                return false;
-            }
-        }
+// A wait that gives up after a number of polls (seconds; a healthy wait takes microseconds). Each poll may sleep in
+// hardware for a while (the hint), so the warps that wait leave the issue slots to the others: without it a tile
+// took 5900 cycles instead of 5100. A role that gave up ends its loop; the others then run into the same
+// limit in their next wait.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < (1 << 22); ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(100000)
+            : "memory");
+        if (ok) return true;
     }
+    raise_fault(WZYB_FAULT_WAIT_TIMEOUT);
+    return false;
 }
+// by a whole warp, which goes on together
+__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, tc_wait(bar, parity));
+}
+
+// the n lowest bits (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
+// One arrival per warp, after all its lanes' work (32 arrivals on one word are taken one after the other).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
+constexpr int kTileMasked = 1, kTileDraft = 2, kTileBad = 4;  // bad: a value scale is infinite or NaN
 
 template <typename T, int HD>
 struct TcSmem {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kRows = 128, kN = 64, NG = HD / 64;
+    static constexpr int kSW = kSplit ? 8 : 16, kParts = kSW / 4;  // softmax warps; lanes per row
+    static constexpr int kThreads = (kSW + 8) * 32;
+    static constexpr int kPairs = (NG + 1) / 2;  // groups are handed on two at a time
     // [group][row][64 dims], 128-byte rows, swizzled
     __half q[kSplit ? 2 : 1][NG][kRows * 64];
     __half k[NG][kN * 64];
     __half v[NG][kN * 64];
     float ks[2][NG][kN], vs[2][NG][kN];
-    float row_scale[kRows];
-    float x_max[2][2][kRows];  // [tile parity][half][row]
-    int x_exp[2][2][kRows];
+    float row_up[kSplit ? kRows : 4];
+    float x_max[2][kParts][kRows];  // [tile parity][part][row]
+    int x_exp[2][kParts][kRows];
     int e_key[2][kN], e_max[2][2];
-    uint64_t k_full, v_full, scales, s_full[NG], p_full[NG], x_full, o_full, done;
+    int4 tile[2];  // position, keys, kTile* flags
+    int bad[2][2];
+    uint64_t k_full, v_full, s_full[kPairs], p_full[kPairs], x_full[4], o_full, done;
     KeyPlan plan;
     uint32_t tmem;
-    int quit;
 };
 
-constexpr int kTcThreads = 512;
-
 template <typename T, int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
     pdl_begin();
     using S = TcSmem<T, HD>;
     constexpr bool kSplit = S::kSplit;
-    constexpr int NG = S::NG, kN = S::kN, kHalf = HD / 2;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    S& sm = *reinterpret_cast<S*>(smem_raw);
+    constexpr int NG = S::NG, kN = S::kN, kSW = S::kSW, kParts = S::kParts, kPairs = S::kPairs, kKeys = kN / kParts, kDims = HD / kParts;
+    extern __shared__ __align__(1024) uint8_t attn_smem[];
+    S& sm = *reinterpret_cast<S*>(attn_smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int split = blockIdx.x, row0 = (gridDim.y - 1 - blockIdx.y) * S::kRows, head = blockIdx.z;
     const int rows = a.T * a.G;
     const int64_t base = (a.d_base_pos ? (int64_t)__ldg(a.d_base_pos) : 0) + a.pos_offset;
 
-    if (warp == 12) {
+    if (warp == kSW + 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else if (warp == 13) {
+    } else if (warp == kSW + 5) {
         build_plan<kN>(a, sm.plan, base, row0 / a.G, (min(row0 + S::kRows, rows) - 1) / a.G + 1, lane);
-    } else if (warp == 14 && lane == 0) {
-        sm.quit = 0;
-        mbar_init(&sm.k_full, 128);
-        mbar_init(&sm.v_full, 128);
-        for (int g = 0; g < NG; ++g) {
-            mbar_init(&sm.s_full[g], 1);
-            mbar_init(&sm.p_full[g], 256);
+    } else if (warp == kSW + 6 && lane == 0) {
+        mbar_init(&sm.k_full, 4);
+        mbar_init(&sm.v_full, 4);
+        for (int i = 0; i < kPairs; ++i) {
+            mbar_init(&sm.s_full[i], i == 0 ? 2 : 1);  // the first also hands the cell warps' scales on
+            mbar_init(&sm.p_full[i], kSW);
         }
-        mbar_init(&sm.scales, 1);
-        mbar_init(&sm.x_full, 256);
+        for (int i = 0; i < 4; ++i) mbar_init(&sm.x_full[i], kParts);
         mbar_init(&sm.o_full, 1);
         mbar_init(&sm.done, 1);
         fence_mbar_init();
-    }
-    if (warp < 12) {  // query rows to shared memory, one warp per row in turn
-        constexpr int kE = HD / 32;
-        for (int r = warp; r < S::kRows; r += 12) {
-            float x[kE];
-            const int row = row0 + r;
-            if (row < rows) {
-                const int t = row / a.G, gq = row - t * a.G;
-                const T* p = static_cast<const T*>(a.q) + t * a.q_row + (int64_t)(head * a.G + gq) * a.q_head + lane * kE;
+    } else if (warp < kSW) {
+        // Query rows to shared memory, a lane 8 elements, kBatch rows of a warp in flight. fp32 rows enter as two
+        // fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range.
+        constexpr int kL = HD / 8, kPer = 32 / kL, kBatch = 4;  // lanes per row, rows per warp instruction
+        const int col = (lane % kL) * 8, g = col / 64, c16 = (col % 64) / 8;
+        for (int r0 = warp * kPer * kBatch; r0 < S::kRows; r0 += kSW * kPer * kBatch) {
+            float x[kBatch][8];
 #pragma unroll
-                for (int i = 0; i < kE; ++i) x[i] = (float)p[i];
-            } else {
+            for (int b = 0; b < kBatch; ++b) {
+                const int row = row0 + r0 + b * kPer + lane / kL;
+                if (row < rows) {
+                    const int t = row / a.G, gq = row - t * a.G;
+                    Vec8<T>::load_ro(static_cast<const T*>(a.q) + t * a.q_row + (int64_t)(head * a.G + gq) * a.q_head + col, x[b]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kE; ++i) x[i] = 0.f;
-            }
-            float f = a.scale_log2;
-            if constexpr (kSplit) {
-                float am = 0.f;
-#pragma unroll
-                for (int i = 0; i < kE; ++i) am = fmaxf(am, fabsf(x[i]));
-                am = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
-                int e = scale_exp(am);
-                if (e < -100 || e > 120) e = 0;
-                const float down = exp2_int(-e);
-                f *= exp2_int(e);
-#pragma unroll
-                for (int i = 0; i < kE; ++i) x[i] *= down;
-            }
-            const int g = lane * kE / 64, c = (lane * kE % 64) * 2;  // byte in the 128-byte row
-            const int at = r * 128 + ((((c >> 4) ^ (r & 7)) << 4) | (c & 15));
-            uint32_t h[kE / 2], l[kE / 2];
-#pragma unroll
-            for (int i = 0; i < kE / 2; ++i) {
-                h[i] = pack_f16(x[2 * i], x[2 * i + 1]);
-                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-                l[i] = pack_f16(x[2 * i] - y.x, x[2 * i + 1] - y.y);
+                    for (int i = 0; i < 8; ++i) x[b][i] = 0.f;
+                }
             }
 #pragma unroll
-            for (int i = 0; i < kE / 2; ++i) {
-                *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at + 4 * i) = h[i];
-                if constexpr (kSplit) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sm.q[kSplit][g]) + at + 4 * i) = l[i];
+            for (int b = 0; b < kBatch; ++b) {
+                const int r = r0 + b * kPer + lane / kL;
+                float f = 1.f;
+                if constexpr (kSplit) {
+                    float am = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[b][i]));
+#pragma unroll
+                    for (int o = kL / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+                    int e = scale_exp(am);
+                    if (e < -100 || e > 120) e = 0;
+                    const float down = exp2_int(-e);
+                    f = exp2_int(e);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[b][i] *= down;
+                }
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h[i] = pack_f16(x[b][2 * i], x[b][2 * i + 1]);
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+                    l[i] = pack_f16(x[b][2 * i] - y.x, x[b][2 * i + 1] - y.y);
+                }
+                const int at = r * 128 + ((c16 ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (kSplit) {
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[kSplit][g]) + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                    if (col == 0) sm.row_up[r] = f;
+                }
             }
-            if (lane == 0) sm.row_scale[r] = f;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -764,64 +815,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
     const KeyPlan& plan = sm.plan;
     const int ntiles = plan.first[plan.ranges];
     const int tb = (int)((int64_t)ntiles * split / a.splits), te = (int)((int64_t)ntiles * (split + 1) / a.splits);
-    const uint32_t tmem = sm.tmem;
-    volatile int* const quit = &sm.quit;
+    // all 512 columns were asked for, so they start at 0; the constant keeps the MMAs' operands immediate
+    constexpr uint32_t tmem = 0;
 
-    if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        const int half = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + r;
+    // registers: launched with 128 (fp32, 512 threads) or 80 (fp16, 768 threads) each; 256 x 208 + 128 x 64 + 128 x 32
+    // and 512 x 96 + 128 x 64 + 128 x 32 are the same totals
+    if (warp < kSW) {
+        if constexpr (kSplit)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+        const int part = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + r, key0 = part * kKeys;
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
+        const uint32_t o_at = mine + 256 + part * kDims;
         const int t = min(row, rows - 1) / a.G;
         const RowSpan span = row_span(a, base, t);
-        const float rs = sm.row_scale[r];
-        float o[kHalf];
+        const float up = kSplit ? sm.row_up[r] : 1.f;
+        float o[kSplit ? kDims : 1];
+        if constexpr (kSplit) {
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) o[i] = 0.f;
+            for (int i = 0; i < kDims; ++i) o[i] = 0.f;
+        }
         float m = -INFINITY, l = 0.f, alpha = 1.f;
         int E = -1000;
         auto unit = [](int e) { return e <= -1000 ? 7 : e; };  // while only scales of 0 have been seen
         bool ok = true;
-        // the previous tile's p V onto o
+        // fp32 calls: the previous tile's p V onto o
         auto drain = [&](uint32_t parity) {
-            ok = __all_sync(0xffffffffu, tc_wait(&sm.o_full, parity, quit));
+            ok = tc_wait_warp(&sm.o_full, parity);
             if (!ok) return;
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < kHalf; c += 16) {
-                float x[16];
-                tc_ld16(x, mine + 256 + half * kHalf + c);
+            for (int c = 0; c < kDims; c += 32) {
+                float x[32];
+                tc_ld16(x, o_at + c);
+                tc_ld16(x + 16, o_at + c + 16);
                 tc_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
+                for (int i = 0; i < 32; i += 2) {
                     const float2 y = ffma2(make_float2(o[c + i], o[c + i + 1]), splat2(alpha), make_float2(x[i], x[i + 1]));
                     o[c + i] = y.x;
                     o[c + i + 1] = y.y;
                 }
             }
         };
-        for (int it = tb; it < te && ok; ++it) {
+        for (int it = tb; it < te; ++it) {
             const int n = it - tb, b = n & 1;
-            if (n > 0) {
-                drain((n - 1) & 1);
-                if (!ok) break;
+            if constexpr (kSplit) {
+                if (n > 0) {
+                    drain(b ^ 1);
+                    if (!ok) break;
+                }
             }
-            ok = __all_sync(0xffffffffu, tc_wait(&sm.scales, b, quit));
-            if (!ok) break;
-            float s[32];
+            float s[kKeys];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = 0.f;
+            for (int i = 0; i < kKeys; ++i) s[i] = 0.f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                ok = ok && __all_sync(0xffffffffu, tc_wait(&sm.s_full[g], b, quit));
-                tc_fence_after();
+                if (g % 2 == 0) {
+                    ok = ok && tc_wait_warp(&sm.s_full[g / 2], b);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
 #pragma unroll
-                for (int c = 0; c < 32; c += 16) {
+                for (int c = 0; c < kKeys; c += 16) {
                     float x[16];
-                    tc_ld16(x, mine + g * 64 + half * 32 + c);
+                    tc_ld16(x, mine + g * 64 + key0 + c);
                     tc_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&sm.ks[b][g][half * 32 + c + i]);
+                        const float4 f = *reinterpret_cast<const float4*>(&sm.ks[b][g][key0 + c + i]);
                         const float2 y0 = ffma2(make_float2(x[i], x[i + 1]), make_float2(f.x, f.y), make_float2(s[c + i], s[c + i + 1]));
                         const float2 y1 = ffma2(make_float2(x[i + 2], x[i + 3]), make_float2(f.z, f.w), make_float2(s[c + i + 2], s[c + i + 3]));
                         s[c + i] = y0.x;
@@ -832,50 +895,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
                 }
             }
             if (!ok) break;
-            const KeyTile kt = key_tile<kN>(plan, it);
-            const bool masked = !tile_unmasked<kN>(plan, kt);  // CTA-uniform
             float top = -INFINITY;
+            const int4 tile = sm.tile[b];
             int e = max(sm.e_max[b][0], sm.e_max[b][1]);
-            if (!masked) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    s[i] *= rs;
-                    top = fmaxf(top, s[i]);
-                }
-            } else {
+            if (tile.z & kTileMasked) {  // CTA-uniform
                 uint32_t see = 0;
-                const int key0 = half * 32;
-                if (kt.draft) {
-                    const int wd = (kt.pos + key0) >> 5;
-                    if (wd < a.mask_words) see = __ldg(a.mask + (int64_t)t * a.mask_words + wd);
-                    if (kt.count < key0 + 32) see &= kt.count > key0 ? (1u << (kt.count - key0)) - 1u : 0u;
+                if (tile.z & kTileDraft) {
+                    const int wd = (tile.x + key0) >> 5;
+                    see = wd < a.mask_words ? __ldg(a.mask + (int64_t)t * a.mask_words + wd) >> (key0 & 31) : 0u;
+                    see &= low_bits(tile.y - key0);
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int pos = kt.pos + key0 + i;
-                        if (key0 + i < kt.count && pos <= span.hi && (pos < plan.sinks || pos > span.lo)) see |= 1u << i;
-                    }
+                    const int p0 = tile.x + key0;
+                    see = (low_bits(span.hi + 1 - p0) & ~low_bits(span.lo + 1 - p0)) | low_bits(min(plan.sinks, span.hi + 1) - p0);
+                    see &= low_bits(tile.y - key0);
                 }
                 e = -1000;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (see >> i & 1u) {
-                        s[i] *= rs;
+                for (int i = 0; i < kKeys; ++i) {
+                    if (see >> i & 1u)
                         e = max(e, sm.e_key[b][key0 + i]);
-                    } else {
+                    else
                         s[i] = -INFINITY;
-                    }
-                    top = fmaxf(top, s[i]);
                 }
+                sm.x_exp[b][part][r] = e;
             }
-            sm.x_max[b][half][r] = top;
-            sm.x_exp[b][half][r] = e;
-            mbar_arrive(&sm.x_full);
-            // also: every score has been read, so weights may take their columns
-            ok = __all_sync(0xffffffffu, tc_wait(&sm.x_full, b, quit));
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) top = fmaxf(top, s[i]);
+            sm.x_max[b][part][r] = top * up;
+            warp_arrive(&sm.x_full[warp & 3], lane);
+            // the warps of these 32 rows; also: their scores have been read, so weights may take their columns
+            ok = tc_wait_warp(&sm.x_full[warp & 3], b);
             if (!ok) break;
-            top = fmaxf(top, sm.x_max[b][half ^ 1][r]);
-            e = max(e, sm.x_exp[b][half ^ 1][r]);
+            top = sm.x_max[b][0][r];
+#pragma unroll
+            for (int i = 1; i < kParts; ++i) top = fmaxf(top, sm.x_max[b][i][r]);
+            if (tile.z & kTileMasked) {
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) e = max(e, sm.x_exp[b][i][r]);
+            }
             alpha = 1.f;
             if (top > m + 8.f || e > E) {
                 top = fmaxf(top, m);
@@ -885,119 +942,183 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
                 m = top;
                 E = e;
             }
+            if constexpr (!kSplit) {
+                if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    ok = tc_wait_warp(&sm.o_full, b ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < kDims; c += 16) {
+                        float x[16];
+                        tc_ld16(x, o_at + c);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] *= alpha;
+                        tc_st16(o_at + c, x);
+                    }
+                }
+            }
             // p * 2^(7 - E), so that p * vs has the weights' size; l sums these
             const float shift = (m == -INFINITY ? 0.f : m) - (float)(7 - unit(E));
-            float sum = 0.f;
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                s[i] = ex2_approx(s[i] - shift);
-                sum += s[i];
+            for (int i = 0; i < kKeys; i += 2) {
+                float2 y = make_float2(s[i], s[i + 1]);
+                y = kSplit ? ffma2(y, splat2(up), splat2(-shift)) : fadd2(y, splat2(-shift));
+                s[i] = ex2_approx(y.x);
+                s[i + 1] = ex2_approx(y.y);
+                sum = fadd2(sum, make_float2(s[i], s[i + 1]));
             }
-            l += sum;
+            l += sum.x + sum.y;
+            // A weight of 0 (a place that the row does not see) stays 0 whatever the cell's scale is: that takes
+            // a comparison per weight, which only tiles with an infinite or NaN scale pay for.
+            auto weights = [&](int g, auto bad) {
+                constexpr int kPiece = kSplit ? 8 : 16;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
+                for (int c = 0; c < kKeys; c += kPiece) {
+                    uint32_t hi[kPiece / 2];
+                    [[maybe_unused]] uint32_t lo[kPiece / 2];
 #pragma unroll
-                for (int c = 0; c < 32; c += 16) {
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&sm.vs[b][g][half * 32 + c + i]);
-                        float w[4] = {s[c + i] * f.x, s[c + i + 1] * f.y, s[c + i + 2] * f.z, s[c + i + 3] * f.w};
-                        if (masked) {  // a weight of 0 stays 0 whatever the cell's scale (infinite or NaN) is
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) w[j] = s[c + i + j] == 0.f ? 0.f : w[j];
+                    for (int i = 0; i < kPiece; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&sm.vs[b][g][key0 + c + i]);
+                        float2 w0 = fmul2(make_float2(s[c + i], s[c + i + 1]), make_float2(f.x, f.y));
+                        float2 w1 = fmul2(make_float2(s[c + i + 2], s[c + i + 3]), make_float2(f.z, f.w));
+                        if constexpr (decltype(bad)::value) {
+                            w0 = make_float2(s[c + i] == 0.f ? 0.f : w0.x, s[c + i + 1] == 0.f ? 0.f : w0.y);
+                            w1 = make_float2(s[c + i + 2] == 0.f ? 0.f : w1.x, s[c + i + 3] == 0.f ? 0.f : w1.y);
                         }
                         if constexpr (kSplit) {
-                            split_f16(w[0], w[1], hi[i / 2], lo[i / 2]);
-                            split_f16(w[2], w[3], hi[i / 2 + 1], lo[i / 2 + 1]);
+                            split_f16(w0.x, w0.y, hi[i / 2], lo[i / 2]);
+                            split_f16(w1.x, w1.y, hi[i / 2 + 1], lo[i / 2 + 1]);
                         } else {
-                            hi[i / 2] = pack_f16(w[0], w[1]);
-                            hi[i / 2 + 1] = pack_f16(w[2], w[3]);
+                            hi[i / 2] = pack_f16(w0.x, w0.y);
+                            hi[i / 2 + 1] = pack_f16(w1.x, w1.y);
                         }
                     }
-                    tc_st8(mine + g * 64 + half * 16 + c / 2, hi);
-                    if constexpr (kSplit) tc_st8(mine + g * 64 + 32 + half * 16 + c / 2, lo);
+                    tc_st(mine + g * 64 + (key0 + c) / 2, hi);
+                    if constexpr (kSplit) tc_st(mine + g * 64 + 32 + (key0 + c) / 2, lo);
                 }
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sm.p_full[g]);
+                if (g % 2 == 1 || g == NG - 1) {
+                    tc_wait_st();
+                    tc_fence_before();
+                    warp_arrive(&sm.p_full[g / 2], lane);
+                }
+            };
+            if (sm.bad[b][0] | sm.bad[b][1]) {
+#pragma unroll 1
+                for (int g = 0; g < NG; ++g) weights(g, std::true_type{});
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) weights(g, std::false_type{});
             }
         }
-        if (te > tb && ok) drain((te - tb - 1) & 1);
-        // the row's sum over both halves of the keys, then its o (or its part of it)
-        sm.x_max[0][half][r] = l;
-        mbar_arrive(&sm.x_full);
-        ok = ok && tc_wait(&sm.x_full, (te - tb) & 1, quit);
-        l += sm.x_max[0][half ^ 1][r];
-        if (row < rows && ok) {
+        if (te > tb && ok) {
+            if constexpr (kSplit) {
+                drain((te - tb - 1) & 1);
+            } else {
+                ok = tc_wait_warp(&sm.o_full, (te - tb - 1) & 1);
+                tc_fence_after();
+            }
+        }
+        // the row's sum over its lanes, then its o
+        sm.x_max[0][part][r] = l;
+        warp_arrive(&sm.x_full[warp & 3], lane);
+        ok = ok && tc_wait_warp(&sm.x_full[warp & 3], (te - tb) & 1);
+        if (ok) {
+            l = sm.x_max[0][0][r];
+#pragma unroll
+            for (int i = 1; i < kParts; ++i) l += sm.x_max[0][i][r];
             const int gq = row - t * a.G, hq = head * a.G + gq;
-            const int64_t orow = (int64_t)t * a.G * a.kv_heads + hq;
+            const int64_t orow = (int64_t)t * a.G * a.kv_heads + hq, at = (int64_t)split * rows * a.kv_heads + orow;
             const float back = exp2_int(unit(E) - 7);  // of l and of o
-            if (a.splits == 1) {
-                const float norm = l == 0.f ? 0.f : 1.f / l;
-                if (half == 0 && a.lse != nullptr)
+            const float norm = a.splits > 1 ? back : (l == 0.f ? 0.f : 1.f / l);
+            if (row < rows && part == 0) {
+                if (a.splits > 1)
+                    a.part_ml[at] = make_float2(m, l * back);
+                else if (a.lse != nullptr)
                     a.lse[orow] = l == 0.f ? -INFINITY : (m + (float)(unit(E) - 7) + log2f(l)) * 0.6931471805599453f;
-                T* const p = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + half * kHalf;
+            }
+            T* const po = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + part * kDims;
+            float* const pp = a.part_o + at * HD + part * kDims;
+#pragma unroll
+            for (int c = 0; c < kDims; c += 16) {
+                float x[16];
                 if constexpr (kSplit) {
 #pragma unroll
-                    for (int i = 0; i < kHalf; i += 4)
-                        *reinterpret_cast<float4*>(p + i) = make_float4(o[i] * norm, o[i + 1] * norm, o[i + 2] * norm, o[i + 3] * norm);
+                    for (int i = 0; i < 16; ++i) x[i] = o[c + i] * norm;
+                } else if (te > tb) {
+                    tc_ld16(x, o_at + c);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = l == 0.f ? 0.f : x[i] * norm;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kHalf; i += 8)
-                        *reinterpret_cast<uint4*>(p + i) =
-                            make_uint4(pack_f16(o[i] * norm, o[i + 1] * norm), pack_f16(o[i + 2] * norm, o[i + 3] * norm),
-                                       pack_f16(o[i + 4] * norm, o[i + 5] * norm), pack_f16(o[i + 6] * norm, o[i + 7] * norm));
+                    for (int i = 0; i < 16; ++i) x[i] = 0.f;
                 }
-            } else {
-                const int64_t at = (int64_t)split * rows * a.kv_heads + orow;
-                if (half == 0) a.part_ml[at] = make_float2(m, l * back);
-                float* const p = a.part_o + at * HD + half * kHalf;
+                if (row >= rows) continue;
+                if (a.splits > 1 || kSplit) {
+                    float* const d = a.splits > 1 ? pp : reinterpret_cast<float*>(po);
 #pragma unroll
-                for (int i = 0; i < kHalf; i += 4)
-                    *reinterpret_cast<float4*>(p + i) = make_float4(o[i] * back, o[i + 1] * back, o[i + 2] * back, o[i + 3] * back);
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4*>(d + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8)
+                        *reinterpret_cast<uint4*>(po + c + i) = make_uint4(pack_f16(x[i], x[i + 1]), pack_f16(x[i + 2], x[i + 3]),
+                                                                           pack_f16(x[i + 4], x[i + 5]), pack_f16(x[i + 6], x[i + 7]));
+                }
             }
         }
-    } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        const int u = tid - 256;
-        constexpr int kCh = HD / 16, kKeys = kN * kCh / 128;  // 16-byte pieces of a row; rows per thread
-        const int c = u % kCh, key0 = u / kCh;
-        uint4 kr[kKeys], vr[kKeys];
-        float sc[NG];  // K scales of key u (u < 64) or V scales of key u - 64
-        int cells[kKeys];
+    } else if (warp < kSW + 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        const int u = tid - kSW * 32;
+        constexpr int kCh = HD / 16, kMine = kN * kCh / 128, kStep = 128 / kCh;  // 16-byte pieces of a row; rows per thread
+        // lanes of odd groups take the neighbouring key, whose swizzle differs in the lowest bit: 8 lanes that store
+        // together use 8 different banks
+        const int c = u % kCh, first = (u / kCh) ^ (c / 4 & 1);
+        const int kvd = a.kv_heads * HD, spc = a.kv_heads * NG;
+        uint4 raw[kMine];  // one tile's K or V pieces: 64 for both would not fit beside the rest
+        uint16_t sc[NG];  // K scales of key u (u < 64) or V scales of key u - 64, converted when they are used
+        // the tile being loaded: its cells are consecutive, but for one step back by `div` where the ring wraps (a
+        // tile holds no more keys than the ring)
+        KeyTile kt;
+        int cell0 = 0;
+        const int div = (int)a.ring_div;
         auto find = [&](int it) {
-            const KeyTile kt = key_tile<kN>(plan, it);
+            kt = key_tile<kN>(plan, it);
+            cell0 = (int)cell_of(a, kt.draft, kt.pos);
+        };
+        auto cell = [&](int key) {
+            const int x = cell0 + key;
+            return !kt.draft && !a.from_full && x >= (int)a.c.ring_cap ? x - div : x;
+        };
+        // the tile's 16-byte pieces into registers; keys past its end get zero codes (and zero scales)
+        auto load = [&](bool value) {
+            const int8_t* const src = (kt.draft ? (value ? a.d.ring_v_q : a.d.ring_k_q)
+                                                : (a.from_full ? (value ? a.c.full_v_q : a.c.full_k_q) : (value ? a.c.ring_v_q : a.c.ring_k_q))) +
+                                      head * HD + c * 16;
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-                const int key = key0 + i * (128 / kCh);
-                cells[i] = key < kt.count ? (int)cell_of(a, kt.draft, kt.pos + key) : -1;
+            for (int i = 0; i < kMine; ++i) {
+                const int key = first + i * kStep;
+                raw[i] = key < kt.count ? __ldg(reinterpret_cast<const uint4*>(src + (int64_t)cell(key) * kvd)) : make_uint4(0, 0, 0, 0);
             }
         };
-        const int kvd = a.kv_heads * HD, spc = a.kv_heads * NG;
-        // keys past the tile's end: zero codes and zero scales
-        auto load = [&](uint4 (&x)[kKeys], int it, bool value) {
-            const bool draft = key_tile<kN>(plan, it).draft;
-            const Planes pl = planes_of<HD>(a, draft, head);
-            const int8_t* const src = (value ? pl.vq : pl.kq) + c * 16;
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-                x[i] = cells[i] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(src + (int64_t)cells[i] * kvd));
-        };
-        auto load_sc = [&](int it) {
-            const KeyTile kt = key_tile<kN>(plan, it);
-            const Planes pl = planes_of<HD>(a, kt.draft, head);
+        auto load_sc = [&]() {
             const int key = u & 63;
+            const bool value = u >= 64;
+            const uint16_t* const src = (kt.draft ? (value ? a.d.ring_v_s : a.d.ring_k_s)
+                                                  : (a.from_full ? (value ? a.c.full_v_s : a.c.full_k_s) : (value ? a.c.ring_v_s : a.c.ring_k_s))) +
+                                        head * NG;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) sc[g] = 0.f;
-            if (key < kt.count) load_scales<NG>((u < 64 ? pl.ks : pl.vs) + cell_of(a, kt.draft, kt.pos + key) * spc, sc);
+            for (int g = 0; g < NG; ++g) sc[g] = 0;
+            if (key < kt.count) load_scale_bits<NG>(src + (int64_t)cell(key) * spc, sc);
         };
-        auto widen = [&](const uint4 (&x)[kKeys], __half (&dst)[NG][kN * 64]) {
+        auto widen = [&](__half (&dst)[NG][kN * 64]) {
             uint8_t* const d = reinterpret_cast<uint8_t*>(dst[c / 4]);
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-                const int key = key0 + i * (128 / kCh), c16 = (c % 4) * 2;
-                const uint32_t w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u};
+            for (int i = 0; i < kMine; ++i) {
+                const int key = first + i * kStep, c16 = (c % 4) * 2;
+                const uint32_t w[4] = {raw[i].x ^ 0x80808080u, raw[i].y ^ 0x80808080u, raw[i].z ^ 0x80808080u, raw[i].w ^ 0x80808080u};
                 *reinterpret_cast<uint4*>(d + key * 128 + ((c16 ^ (key & 7)) << 4)) =
                     make_uint4(codes_f16(w[0], kSelLo), codes_f16(w[0], kSelHi), codes_f16(w[1], kSelLo), codes_f16(w[1], kSelHi));
                 *reinterpret_cast<uint4*>(d + key * 128 + (((c16 + 1) ^ (key & 7)) << 4)) =
@@ -1008,51 +1129,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
         bool ok = true;
         if (tb < te) {
             find(tb);
-            load_sc(tb);
-            load(kr, tb, false);
-            load(vr, tb, true);
+            load_sc();
+            load(false);
         }
         for (int it = tb; it < te; ++it) {
             const int n = it - tb, b = n & 1;
-            if (n > 0) ok = __all_sync(0xffffffffu, tc_wait(&sm.s_full[NG - 1], b ^ 1, quit));  // K's memory is free
+            if (n > 0) ok = tc_wait_warp(&sm.s_full[kPairs - 1], b ^ 1);  // K's memory is free
             if (!ok) break;
             int e = -1000;
+            bool bad = false;
+            const float f = u < 64 ? a.scale_log2 : 1.f;  // scores in log2 units
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                (u < 64 ? sm.ks : sm.vs)[b][g][u & 63] = sc[g];
-                e = max(e, scale_exp(sc[g]));
+                const float x = __half2float(__ushort_as_half(sc[g]));
+                (u < 64 ? sm.ks : sm.vs)[b][g][u & 63] = x * f;
+                e = max(e, scale_exp(x));
+                bad = bad || !(fabsf(x) <= 65504.f);
             }
             if (u >= 64) {
                 sm.e_key[b][u - 64] = e;
                 e = __reduce_max_sync(0xffffffffu, e);
                 if (lane == 0) sm.e_max[b][(u - 64) >> 5] = e;
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane == 0) sm.bad[b][(u - 64) >> 5] = bad ? kTileBad : 0;
             }
-            widen(kr, sm.k);
-            mbar_arrive(&sm.k_full);
+            if (u == 0)
+                sm.tile[b] = make_int4(kt.pos, kt.count, (tile_unmasked<kN>(plan, kt) ? 0 : kTileMasked) | (kt.draft ? kTileDraft : 0), 0);
+            widen(sm.k);
+            warp_arrive(&sm.k_full, lane);
+            load(true);
+            if (n > 0) ok = tc_wait_warp(&sm.o_full, b ^ 1);  // V's memory is free
+            if (!ok) break;
+            widen(sm.v);
+            warp_arrive(&sm.v_full, lane);
             if (it + 1 < te) {
                 find(it + 1);
-                load_sc(it + 1);
-                load(kr, it + 1, false);
+                load_sc();
+                load(false);
             }
-            if (n > 0) ok = __all_sync(0xffffffffu, tc_wait(&sm.o_full, b ^ 1, quit));  // V's memory is free
-            if (!ok) break;
-            widen(vr, sm.v);
-            mbar_arrive(&sm.v_full);
-            if (it + 1 < te) load(vr, it + 1, true);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-        if (warp == 12 && lane == 0 && tb < te) {
+        if (warp == kSW + 4 && tb < te) {  // the whole warp, converged; one lane issues
             const uint64_t qd = tc_desc(smem_u32(sm.q[0][0])), ql = tc_desc(smem_u32(sm.q[kSplit ? 1 : 0][0]));
             const uint64_t kd = tc_desc(smem_u32(sm.k[0])), vd = tc_desc(smem_u32(sm.v[0]));
             constexpr uint64_t kQG = S::kRows * 128 >> 4, kKG = kN * 128 >> 4;  // a group's bytes in descriptor units
             bool ok = true;
             for (int n = 0; n < te - tb && ok; ++n) {
                 const int b = n & 1;
-                if (n > 0) ok = tc_wait(&sm.o_full, b ^ 1, quit);  // the weights' columns are free
-                ok = ok && tc_wait(&sm.k_full, b, quit);
+                ok = tc_wait_warp(&sm.k_full, b);
+                if (n > 0) ok = ok && tc_wait_warp(&sm.o_full, b ^ 1);  // the weights' columns are free
                 if (!ok) break;
-                mbar_arrive(&sm.scales);  // hands the cell warps' scales on to the softmax warps
+                if (lane == 0) mbar_arrive(&sm.s_full[0]);
                 tc_fence_after();
 #pragma unroll 1
                 for (int g = 0; g < NG; ++g) {
@@ -1064,14 +1192,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
                         for (int x = 0; x < 4; ++x)
                             tc_mma_ss(tmem + g * 64, ql + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, 1);
                     }
-                    tc_commit(&sm.s_full[g]);
+                    if (g % 2 == 1 || g == NG - 1) tc_commit(&sm.s_full[g / 2]);
                 }
-                ok = tc_wait(&sm.v_full, b, quit);
+                ok = tc_wait_warp(&sm.v_full, b);
 #pragma unroll 1
                 for (int g = 0; g < NG; ++g) {
-                    ok = ok && tc_wait(&sm.p_full[g], b, quit);
-                    if (!ok) break;
-                    tc_fence_after();
+                    if (g % 2 == 0) {
+                        ok = ok && tc_wait_warp(&sm.p_full[g / 2], b);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
                     const uint32_t d = tmem + 256 + g * 64, p = tmem + g * 64;
                     if constexpr (kSplit) {
 #pragma unroll
@@ -1079,7 +1209,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
                             tc_mma_ts(d, p + 32 + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, x > 0);
                         tc_mma_ts_down11(d, p, vd + g * kKG, kTcIdescBMn);
                     } else {
-                        tc_mma_ts(d, p, vd + g * kKG, kTcIdescBMn, 0);
+                        tc_mma_ts(d, p, vd + g * kKG, kTcIdescBMn, n > 0);
                     }
 #pragma unroll
                     for (int x = 1; x < 4; ++x) tc_mma_ts(d, p + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, 1);
@@ -1094,7 +1224,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tile_kernel(const KvAtt
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == kSW + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // Joins the splits' parts of one row per CTA, in split order: HD / 4 lanes of 4 elements, the other threads
@@ -1189,7 +1319,7 @@ static int launch_attn(KvAttnArgs& a, const AttnShape& s, cudaStream_t stream) {
         const int smem = (int)sizeof(TcSmem<T, HD>);
         rc = ensure_smem((const void*)kern, smem);
         if (rc != WZYB_OK) return rc;
-        launch_k(kern, grid, kTcThreads, smem, stream, a);
+        launch_k(kern, grid, TcSmem<T, HD>::kThreads, smem, stream, a);
     }
     if (a.splits > 1) launch_k(kv_attn_join_kernel<T, HD>, a.T * a.G * a.kv_heads, 256, 0, stream, a);
     return launch_status();
@@ -1215,7 +1345,7 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     if (tree && (!drafts || !mask || !depth || !drafts->ring_k_q || !drafts->ring_k_s || !drafts->ring_v_q ||
                  !drafts->ring_v_s))
         return WZYB_ERR_NULL;
-    constexpr int64_t kMaxPos = 0x7FFFFFFF;
+    constexpr int64_t kMaxPos = 0x40000000;  // positions and cells are ints, with room for a tile past them
     if (T_ < 0 || T_ > (1 << 22) || x.kv_heads < 1 || x.kv_heads > 64 || x.q_heads < 1 || x.q_heads > 256 ||
         x.q_heads % x.kv_heads != 0 || (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) ||
         x.window < 0 || x.sinks < 0 || c.max_ctx < 0 || c.max_ctx > kMaxPos ||
