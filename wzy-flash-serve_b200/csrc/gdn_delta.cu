@@ -597,12 +597,31 @@ __device__ __forceinline__ void gdn_operand(const float (&x)[N][4], const int (&
         }
 }
 
-// One warp owns 8 value columns of a head from the first chunk to the last: its part of S stays in its
-// registers as fp32 accumulator tiles, and S, X = V - e^G K S and d = T X pass from product to product inside the
-// warp (columns never mix), so the chunk's chain needs no barrier. The four warps of a CTA share the
-// chunk's K, Q, T and P in shared memory, fetched by cp.async while the chunk before is worked through.
+// What a state warp hands to its output warp, as second operands (16 bytes per lane and index): S at the chunk's
+// start and d, each with the scales of its two columns per lane.
+template <int HD>
+struct GdnHandOver {
+    uint4 s[HD / 16][32];  // per step of 16: hi, hi, lo, lo
+    uint4 d[4][32];
+    float2 s_up[32], d_up[32];
+};
+template <int N>
+__device__ __forceinline__ void gdn_hand(uint4 (&to)[N][32], const uint32_t (&hi)[N][2], const uint32_t (&lo)[N][2], int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i][lane] = make_uint4(hi[i][0], hi[i][1], lo[i][0], lo[i][1]);
+}
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// 8 value columns of a head belong to two warps from the first chunk to the last. The state warp keeps its part of S
+// in its registers as fp32 accumulator tiles; S, X = V - e^G K S and d = T X pass from product to product inside it
+// (columns never mix), so its chain, which is what the chunks wait for, needs no barrier but the one per chunk. The
+// output warp takes S and d from it as operands and makes o = e^G Q S + P d meanwhile (one warp for both
+// took 1.5 times as long: the chain leaves most issue slots empty). The CTA's four pairs share the chunk's K, Q, T
+// and P in shared memory, fetched by cp.async while the chunk before is worked through.
 template <typename T, int HD>
-__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
+__global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
     pdl_begin();
     using Stage = GdnScanStage<T, HD>;
     constexpr bool kSplit = Stage::kSplit;
@@ -610,7 +629,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Stage* const st = reinterpret_cast<Stage*>(smem_raw);
     const GdnDeltaArgs& a = p.x;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, pair = (tid >> 5) & 3, g = lane >> 2, t4 = lane & 3;
+    const bool out_warp = tid >= 128;
+    GdnHandOver<HD>& hand = reinterpret_cast<GdnHandOver<HD>*>(smem_raw + 2 * sizeof(Stage))[pair];
     const int h = blockIdx.x / (HD / 32), c0 = (blockIdx.x % (HD / 32)) * 32;
     const int hk = h / (a.v_heads / a.k_heads);
     const int chunks = (int)((p.t1 - p.t0 + kGdnChunk - 1) / kGdnChunk);
@@ -623,26 +644,32 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
         if constexpr (kSplit) {
             const __half* const src = p.kq + ((int64_t)ch * a.k_heads + hk) * (4 * 64 * HD);
 #pragma unroll 4
-            for (int i = tid; i < 4 * 64 * kRowChunks; i += 128) {
+            for (int i = tid; i < 4 * 64 * kRowChunks; i += 256) {
                 const int m = i / (64 * kRowChunks), r = (i / kRowChunks) % 64, c = (i % kRowChunks) * 8;
                 __half* const base = m < 2 ? s.k[m & 1] : s.q[m & 1];
                 cp_async16(base + r * kLd + c, src + (m * 64 + r) * HD + c);
             }
         } else {
-#pragma unroll 4
-            for (int i = tid; i < 2 * 64 * kRowChunks; i += 128) {
-                const int m = i / (64 * kRowChunks), r = (i / kRowChunks) % 64, c = (i % kRowChunks) * 8;
-                __half* const dst = (m ? s.q[0] : s.k[0]) + r * kLd + c;
-                const __half* const src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r) * (m ? a.q_row : a.k_row) + hk * HD + c;
-                if (r < n)
-                    cp_async16(dst, src);
-                else
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            // a thread keeps its piece of the row; rows go up by 256 / pieces
+            const int c = (tid % kRowChunks) * 8, r0 = tid / kRowChunks;
+            constexpr int kStep = 256 / kRowChunks;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int64_t row = m ? a.q_row : a.k_row;
+                const __half* src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r0) * row + hk * HD + c;
+                __half* dst = (m ? s.q[0] : s.k[0]) + r0 * kLd + c;
+#pragma unroll
+                for (int r = r0; r < 64; r += kStep, src += kStep * row, dst += kStep * kLd) {
+                    if (r < n)
+                        cp_async16(dst, src);
+                    else
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+                }
             }
         }
         constexpr int kVC = 32 * sizeof(T) / 16, kVE = 16 / sizeof(T);
 #pragma unroll
-        for (int i = tid; i < 64 * kVC; i += 128) {
+        for (int i = tid; i < 64 * kVC; i += 256) {
             const int r = i / kVC, c = (i % kVC) * kVE;
             T* const dst = s.v + r * kVLd + c;
             if (r < n)
@@ -652,12 +679,79 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
         }
         const uint4* const src = reinterpret_cast<const uint4*>(p.data + ((int64_t)ch * a.v_heads + h) * sizeof(GdnChunkData<kSplit>));
         uint4* const dst = reinterpret_cast<uint4*>(&s.d);
-#pragma unroll 4
-        for (int i = tid; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 128) cp_async16(dst + i, src + i);
+#pragma unroll
+        for (int i = tid; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 256) cp_async16(dst + i, src + i);
         cp_async_commit();
     };
 
-    const int col = c0 + warp * 8 + 2 * t4;  // this lane's columns col, col + 1
+    const int col = c0 + pair * 8 + 2 * t4;  // this lane's columns col, col + 1
+    const int arow = lane & 15, acol = (lane >> 4) * 8;
+    fetch(0);
+    if (out_warp) {
+        for (int ch = 0; ch < chunks; ++ch) {
+            cp_async_wait<0>();
+            __syncthreads();  // chunk ch is there for all, and nobody still reads the other buffers
+            if (ch + 1 < chunks) fetch(ch + 1);
+            const Stage& z = st[ch & 1];
+            named_bar_sync(1 + pair, 64);  // S
+            uint4 so[kM];
+#pragma unroll
+            for (int i = 0; i < kM; ++i) so[i] = hand.s[i][lane];
+            const float2 su = hand.s_up[lane];
+            float o[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float qh[4] = {}, ql[4] = {};
+#pragma unroll
+                for (int ks = 0; ks < kM; ++ks) {
+                    uint32_t fq[4];
+                    ldmatrix_x4(fq, z.q[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                    mma_f16(qh, fq, so[ks].x, so[ks].y);
+                    mma_f16(ql, fq, so[ks].z, so[ks].w);
+                    if constexpr (kSplit) {
+                        ldmatrix_x4(fq, z.q[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                        mma_f16(ql, fq, so[ks].x, so[ks].y);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    o[i][c] = z.d.b[16 * i + g + (c >> 1) * 8] * (c & 1 ? su.y : su.x) * fmaf(ql[c], 1.f / kGdnLo, qh[c]);
+            }
+            named_bar_sync(5 + pair, 64);  // d
+            uint4 dd[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dd[i] = hand.d[i][lane];
+            const float2 du = hand.d_up[lane];
+            const float2 up = make_float2(du.x * z.d.p_up, du.y * z.d.p_up);
+            const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float oh[4] = {}, ol[4] = {};
+#pragma unroll
+                for (int j = 0; j <= i; ++j) {
+                    const uint4 ph = z.d.p[i * (i + 1) / 2 + j][lane];
+                    mma_f16(oh, ph, dd[j].x, dd[j].y);
+                    mma_f16(ol, ph, dd[j].z, dd[j].w);
+                    if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dd[j].x, dd[j].y);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[i][c] = fmaf(c & 1 ? up.y : up.x, fmaf(ol[c], 1.f / kGdnLo, oh[c]), o[i][c]);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int64_t t = tok0 + 16 * i + g + 8 * b;
+                    if (t < p.t1) {
+                        T* const dst = static_cast<T*>(a.o) + t * a.o_row + h * HD + col;
+                        if constexpr (kSplit)
+                            *reinterpret_cast<float2*>(dst) = make_float2(o[i][2 * b], o[i][2 * b + 1]);
+                        else
+                            *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(o[i][2 * b], o[i][2 * b + 1]);
+                    }
+                }
+            }
+        }
+        return;
+    }
+
     float s[kM][4];  // S: rows k = 16*i + g, + 8
     const float* const sin = p.state_in + ((int64_t)h * HD + col) * HD;
 #pragma unroll
@@ -665,12 +759,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             s[i][c] = p.state_in != nullptr ? sin[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] : 0.f;
-    int es[2] = {0, 0}, ex[2] = {0, 0}, ed[2] = {0, 0};
-
-    fetch(0);
+    int es[2] = {0, 0}, ex[2] = {0, 0}, ed[2] = {0, 0}, ec[2] = {0, 0};
     for (int ch = 0; ch < chunks; ++ch) {
         cp_async_wait<0>();
-        __syncthreads();  // chunk ch is there for all, and nobody still reads the other buffer
+        __syncthreads();
         if (ch + 1 < chunks) fetch(ch + 1);
         const Stage& z = st[ch & 1];
         const bool force = (ch & 15) == 0;
@@ -679,34 +771,34 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
         gdn_col_exp(s, es, force);
         gdn_operand(s, es, sh, sl);
         const float su[2] = {gdn_exp2i(es[0]), gdn_exp2i(es[1])};
-        float x[4][4], o[4][4];
-        const int arow = lane & 15, acol = (lane >> 4) * 8;
+        gdn_hand(hand.s, sh, sl, lane);
+        hand.s_up[lane] = make_float2(su[0], su[1]);
+        named_bar_arrive(1 + pair, 64);
+        float x[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float kh[4] = {}, kl[4] = {}, qh[4] = {}, ql[4] = {};
+        for (int i = 0; i < 4; i += 2) {  // two row tiles at a time: four independent chains of products
+            float kh[2][4] = {}, kl[2][4] = {};
 #pragma unroll
-            for (int ks = 0; ks < kM; ++ks) {
-                uint32_t fk[4], fq[4];
-                ldmatrix_x4(fk, z.k[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
-                ldmatrix_x4(fq, z.q[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
-                mma_f16(kh, fk, sh[ks][0], sh[ks][1]);
-                mma_f16(qh, fq, sh[ks][0], sh[ks][1]);
-                mma_f16(kl, fk, sl[ks][0], sl[ks][1]);
-                mma_f16(ql, fq, sl[ks][0], sl[ks][1]);
-                if constexpr (kSplit) {
-                    ldmatrix_x4(fk, z.k[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
-                    ldmatrix_x4(fq, z.q[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
-                    mma_f16(kl, fk, sh[ks][0], sh[ks][1]);
-                    mma_f16(ql, fq, sh[ks][0], sh[ks][1]);
+            for (int ks = 0; ks < kM; ++ks)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t fk[4];
+                    ldmatrix_x4(fk, z.k[0] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
+                    mma_f16(kh[j], fk, sh[ks][0], sh[ks][1]);
+                    mma_f16(kl[j], fk, sl[ks][0], sl[ks][1]);
+                    if constexpr (kSplit) {
+                        ldmatrix_x4(fk, z.k[kSplit] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
+                        mma_f16(kl[j], fk, sh[ks][0], sh[ks][1]);
+                    }
                 }
-            }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int r = 16 * i + g + (c >> 1) * 8;
-                const float v = (float)z.v[r * kVLd + warp * 8 + 2 * t4 + (c & 1)];
-                x[i][c] = v - z.d.a[r] * su[c & 1] * fmaf(kl[c], 1.f / kGdnLo, kh[c]);
-                o[i][c] = z.d.b[r] * su[c & 1] * fmaf(ql[c], 1.f / kGdnLo, qh[c]);
-            }
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int r = 16 * (i + j) + g + (c >> 1) * 8;
+                    const float v = (float)z.v[r * kVLd + pair * 8 + 2 * t4 + (c & 1)];
+                    x[i + j][c] = v - z.d.a[r] * su[c & 1] * fmaf(kl[j][c], 1.f / kGdnLo, kh[j][c]);
+                }
         }
         // d = T X
         uint32_t xh[4][2], xl[4][2];
@@ -716,74 +808,54 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
         float d[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float dh[4] = {}, dl[4] = {};
+            float dh[4] = {}, dl[4] = {}, dm[4] = {};
 #pragma unroll
             for (int j = 0; j <= i; ++j) {
                 const uint4 th = z.d.t_hi[i * (i + 1) / 2 + j][lane], tl = z.d.t_lo[i * (i + 1) / 2 + j][lane];
                 mma_f16(dh, th, xh[j][0], xh[j][1]);
                 mma_f16(dl, th, xl[j][0], xl[j][1]);
-                mma_f16(dl, tl, xh[j][0], xh[j][1]);
+                mma_f16(dm, tl, xh[j][0], xh[j][1]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) d[i][c] = xu[c & 1] * fmaf(dl[c], 1.f / kGdnLo, dh[c]);
+            for (int c = 0; c < 4; ++c) d[i][c] = xu[c & 1] * fmaf(dl[c] + dm[c], 1.f / kGdnLo, dh[c]);
         }
-        // o += P d
         uint32_t dh[4][2], dl[4][2];
         gdn_col_exp(d, ed, force);
         gdn_operand(d, ed, dh, dl);
-        const float du[2] = {gdn_exp2i(ed[0]), gdn_exp2i(ed[1])};
-        const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float oh[4] = {}, ol[4] = {};
-#pragma unroll
-            for (int j = 0; j <= i; ++j) {
-                const uint4 ph = z.d.p[i * (i + 1) / 2 + j][lane];
-                mma_f16(oh, ph, dh[j][0], dh[j][1]);
-                mma_f16(ol, ph, dl[j][0], dl[j][1]);
-                if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dh[j][0], dh[j][1]);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                o[i][c] = fmaf(z.d.p_up * du[c & 1], fmaf(ol[c], 1.f / kGdnLo, oh[c]), o[i][c]);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int64_t t = tok0 + 16 * i + g + 8 * b;
-                if (t < p.t1) {
-                    T* const dst = static_cast<T*>(a.o) + t * a.o_row + h * HD + col;
-                    if constexpr (kSplit)
-                        *reinterpret_cast<float2*>(dst) = make_float2(o[i][2 * b], o[i][2 * b + 1]);
-                    else
-                        *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(o[i][2 * b], o[i][2 * b + 1]);
-                }
-            }
-        }
+        gdn_hand(hand.d, dh, dl, lane);
+        hand.d_up[lane] = make_float2(gdn_exp2i(ed[0]), gdn_exp2i(ed[1]));
+        named_bar_arrive(5 + pair, 64);
         // S <- e^G S + K^T (c d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) d[i][c] *= z.d.c[16 * i + g + (c >> 1) * 8];
-        gdn_col_exp(d, ed, force);
-        gdn_operand(d, ed, dh, dl);
-        const float cu[2] = {gdn_exp2i(ed[0]), gdn_exp2i(ed[1])};
+        gdn_col_exp(d, ec, force);
+        gdn_operand(d, ec, dh, dl);
+        const float cu[2] = {gdn_exp2i(ec[0]), gdn_exp2i(ec[1])};
+        const float decay = z.d.decay;
         const int krow = (lane & 7) + ((lane >> 4) << 3), kcol = ((lane >> 3) & 1) * 8;
 #pragma unroll
-        for (int i = 0; i < kM; ++i) {
-            float nh[4] = {}, nl[4] = {};
+        for (int i = 0; i < kM; i += 2) {
+            float nh[2][4] = {}, nl[2][4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t fk[4];
-                ldmatrix_x4_t(fk, z.k[0] + (j * 16 + krow) * kLd + i * 16 + kcol);
-                mma_f16(nh, fk, dh[j][0], dh[j][1]);
-                mma_f16(nl, fk, dl[j][0], dl[j][1]);
-                if constexpr (kSplit) {
-                    ldmatrix_x4_t(fk, z.k[kSplit] + (j * 16 + krow) * kLd + i * 16 + kcol);
-                    mma_f16(nl, fk, dh[j][0], dh[j][1]);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t fk[4];
+                    ldmatrix_x4_t(fk, z.k[0] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
+                    mma_f16(nh[e], fk, dh[j][0], dh[j][1]);
+                    mma_f16(nl[e], fk, dl[j][0], dl[j][1]);
+                    if constexpr (kSplit) {
+                        ldmatrix_x4_t(fk, z.k[kSplit] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
+                        mma_f16(nl[e], fk, dh[j][0], dh[j][1]);
+                    }
                 }
-            }
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                s[i][c] = fmaf(z.d.decay, s[i][c], cu[c & 1] * fmaf(nl[c], 1.f / kGdnLo, nh[c]));
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    s[i + e][c] = fmaf(decay, s[i + e][c], cu[c & 1] * fmaf(nl[e][c], 1.f / kGdnLo, nh[e][c]));
         }
     }
     float* const sout = a.state_out + ((int64_t)h * HD + col) * HD;
@@ -794,14 +866,15 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 2 : 1) gdn_chunk_scan_ke
 }
 
 // Tokens per segment: what the prep kernel writes for a segment is still in L2 when the scan reads it.
-constexpr int64_t kGdnSegBytes = int64_t(64) << 20;
+constexpr int64_t kGdnSegBytes = int64_t(96) << 20;
 static int64_t gdn_chunk_bytes(bool f32, int k_heads, int v_heads, int head_dim) {
     return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * (int64_t)(4 * 64 * head_dim * 2)
                : v_heads * (int64_t)sizeof(GdnChunkData<false>);
 }
 static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
     const int64_t n = kGdnSegBytes / gdn_chunk_bytes(f32, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
-    return n < 1 ? 1 : (n < all ? n : all);
+    const int64_t segs = n < 1 ? all : (all + n - 1) / n;
+    return segs < 1 ? 1 : (all + segs - 1) / segs;  // segments of one size: a short last one costs as much as a long one's start
 }
 // Calls of at least this many tokens take the chunked form.
 constexpr int64_t kGdnChunkedFrom = 64;
@@ -812,7 +885,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
     const int64_t seg = gdn_seg_chunks(kSplit, a.T, a.k_heads, a.v_heads, HD);
     const auto prep = gdn_chunk_prep_kernel<T, HD>;
     const auto scan = gdn_chunk_scan_kernel<T, HD>;
-    const int prep_smem = (int)sizeof(GdnPrepSmem<T, HD>), scan_smem = (int)(2 * sizeof(GdnScanStage<T, HD>));
+    const int prep_smem = (int)sizeof(GdnPrepSmem<T, HD>), scan_smem = (int)(2 * sizeof(GdnScanStage<T, HD>) + 4 * sizeof(GdnHandOver<HD>));
     int rc = ensure_smem((const void*)prep, prep_smem);
     if (rc == WZYB_OK) rc = ensure_smem((const void*)scan, scan_smem);
     if (rc != WZYB_OK) return rc;
@@ -830,7 +903,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
         sa.t1 = t1;
         const int64_t chunks = (t1 - t0 + kGdnChunk - 1) / kGdnChunk;
         launch_k(prep, (unsigned)(chunks * a.k_heads), 128, prep_smem, stream, pa);
-        launch_k(scan, a.v_heads * (HD / 32), 128, scan_smem, stream, sa);
+        launch_k(scan, a.v_heads * (HD / 32), 256, scan_smem, stream, sa);
         sa.state_in = a.state_out;
     }
     return launch_status();

@@ -201,14 +201,6 @@ __device__ __forceinline__ void load_scale_bits(const uint16_t* p, uint16_t (&s)
         s[0] = __ldg(p);
     }
 }
-template <int NG>
-__device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[NG]) {
-    uint16_t u[NG];
-    load_scale_bits<NG>(p, u);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) s[g] = __half2float(__ushort_as_half(u[g]));
-}
-
 // Two int8 codes as fp16, exactly: with the sign bit flipped (u = c + 128) the byte under the high byte
 // 0x64 is the fp16 number 1024 + u, and 1024 + u - 1152 = c. `sel` picks the bytes of flipped word w.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
@@ -347,36 +339,51 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     int E[2] = {-1000, -1000};
 
-    for (int it = tb + warp; it < te; it += kWarps) {
-        const KeyTile kt = key_tile<kN>(plan, it);
-        const Planes pl = planes_of<HD>(a, kt.draft, head);
-        // lanes 0..15 find the tile's cells; a key past the tile's end takes the first one's cell (its
-        // scales count as 0 and its scores as -inf)
+    // K of the next tile is on its way while the current one is worked through (its registers are free once the
+    // scores are there); V of the current one while its scores are computed.
+    KeyTile kt = {};
+    int my_cell = 0;
+    uint4 kr[2][NG];
+    uint16_t ksb[2][NG];
+    auto load_k = [&](int it) {
+        kt = key_tile<kN>(plan, it);
+        // lanes 0..15 find the tile's cells; a key past the tile's end takes the first one's cell (its scales
+        // count as 0 and its scores as -inf)
         const int mine = lane & 15;
-        const int my_cell = (int)cell_of(a, kt.draft, kt.pos + (mine < kt.count ? mine : 0));
-        int kcell[2], vcell[4];
+        my_cell = (int)cell_of(a, kt.draft, kt.pos + (mine < kt.count ? mine : 0));
+        const Planes pl = planes_of<HD>(a, kt.draft, head);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) kcell[i] = __shfl_sync(0xffffffffu, my_cell, g + 8 * i);
+        for (int i = 0; i < 2; ++i) {
+            const int cell = __shfl_sync(0xffffffffu, my_cell, g + 8 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vcell[i] = __shfl_sync(0xffffffffu, my_cell, 2 * t4 + (i & 1) + (i >> 1) * 8);
-        uint4 kr[2][NG];
+            for (int n = 0; n < NG; ++n)
+                kr[i][n] = __ldg(reinterpret_cast<const uint4*>(pl.kq + (int64_t)cell * kvd + n * 64 + t4 * 16));
+            load_scale_bits<NG>(pl.ks + (int64_t)cell * spc, ksb[i]);
+        }
+    };
+    if (tb + warp < te) load_k(tb + warp);
+    for (int it = tb + warp; it < te; it += kWarps) {
+        const KeyTile now = kt;
         uint2 vr[4][NG];
+        uint16_t vsb[2][NG];
+        float ks[2][NG], vs[2][NG];
+        {
+            const Planes pl = planes_of<HD>(a, now.draft, head);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int cell = __shfl_sync(0xffffffffu, my_cell, 2 * t4 + (i & 1) + (i >> 1) * 8);
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+                    vr[i][n] = __ldg(reinterpret_cast<const uint2*>(pl.vq + (int64_t)cell * kvd + n * 64 + g * 8));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                load_scale_bits<NG>(pl.vs + (int64_t)__shfl_sync(0xffffffffu, my_cell, g + 8 * i) * spc, vsb[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int n = 0; n < NG; ++n)
-                kr[i][n] = __ldg(reinterpret_cast<const uint4*>(pl.kq + (int64_t)kcell[i] * kvd + n * 64 + t4 * 16));
-        float ks[2][NG], vs[2][NG];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            load_scales<NG>(pl.ks + (int64_t)kcell[i] * spc, ks[i]);
-            load_scales<NG>(pl.vs + (int64_t)kcell[i] * spc, vs[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-                vr[i][n] = __ldg(reinterpret_cast<const uint2*>(pl.vq + (int64_t)vcell[i] * kvd + n * 64 + g * 8));
+            for (int n = 0; n < NG; ++n) ks[i][n] = __half2float(__ushort_as_half(ksb[i][n]));
 
         // scores of keys g and g + 8 for rows 2*t4, 2*t4 + 1: s[0], s[1] and s[2], s[3]
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -406,6 +413,11 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[c] = fmaf(acc[c], ks[c >> 1][n], s[c]);
         }
+        if (it + kWarps < te) load_k(it + kWarps);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < NG; ++n) vs[i][n] = __half2float(__ushort_as_half(vsb[i][n]));
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[c] *= rs[c & 1];
         int ek[2] = {-1000, -1000}, e[2];
@@ -413,15 +425,15 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int n = 0; n < NG; ++n) ek[i] = max(ek[i], scale_exp(vs[i][n]));
-        if (tile_unmasked<kN>(plan, kt)) {  // warp-uniform
+        if (tile_unmasked<kN>(plan, now)) {  // warp-uniform
             e[0] = e[1] = max(ek[0], ek[1]);
         } else {
             e[0] = e[1] = -1000;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int key = g + (c >> 1) * 8, pos = kt.pos + key;
-                bool see = key < kt.count;
-                if (kt.draft) {
+                const int key = g + (c >> 1) * 8, pos = now.pos + key;
+                bool see = key < now.count;
+                if (now.draft) {
                     if (see) see = (__ldg(a.mask + (int64_t)rt[c & 1] * a.mask_words + (pos >> 5)) >> (pos & 31)) & 1u;
                 } else {
                     see = see && pos <= span[c & 1].hi && (pos < plan.sinks || pos > span[c & 1].lo);
@@ -757,53 +769,58 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
         mbar_init(&sm.o_full, 1);
         mbar_init(&sm.done, 1);
         fence_mbar_init();
-    } else if (warp < kSW) {
-        // Query rows to shared memory, a lane 8 elements, kBatch rows of a warp in flight. fp32 rows enter as two
-        // fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range.
-        constexpr int kL = HD / 8, kPer = 32 / kL, kBatch = 4;  // lanes per row, rows per warp instruction
+    }
+    if (warp < kSW) {
+        // Query rows to shared memory, a lane 8 elements, all of a warp's rows in flight (two turns for fp32). fp32
+        // rows enter as two fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range.
+        constexpr int kL = HD / 8, kPer = 32 / kL, kMineQ = S::kRows / kSW / kPer;  // lanes per row, rows at a time, loads
+        constexpr int kBatch = kMineQ < 8 ? kMineQ : 8;
         const int col = (lane % kL) * 8, g = col / 64, c16 = (col % 64) / 8;
-        for (int r0 = warp * kPer * kBatch; r0 < S::kRows; r0 += kSW * kPer * kBatch) {
-            float x[kBatch][8];
+#pragma unroll 1
+        for (int r0 = warp * kPer * kMineQ; r0 < (warp + 1) * kPer * kMineQ; r0 += kPer * kBatch) {
+            uint4 raw[kBatch][sizeof(T) / 2];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int row = row0 + r0 + b * kPer + lane / kL;
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[b][i] = make_uint4(0, 0, 0, 0);
                 if (row < rows) {
                     const int t = row / a.G, gq = row - t * a.G;
-                    Vec8<T>::load_ro(static_cast<const T*>(a.q) + t * a.q_row + (int64_t)(head * a.G + gq) * a.q_head + col, x[b]);
-                } else {
+                    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + t * a.q_row +
+                                                                          (int64_t)(head * a.G + gq) * a.q_head + col);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[b][i] = 0.f;
+                    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[b][i] = __ldg(p + i);
                 }
             }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int r = r0 + b * kPer + lane / kL;
-                float f = 1.f;
-                if constexpr (kSplit) {
+                const int at = r * 128 + ((c16 ^ (r & 7)) << 4);
+                if constexpr (!kSplit) {
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at) = raw[b][0];
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const float*>(&raw[b][0])[i];
                     float am = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[b][i]));
+                    for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[i]));
 #pragma unroll
                     for (int o = kL / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
                     int e = scale_exp(am);
                     if (e < -100 || e > 120) e = 0;
                     const float down = exp2_int(-e);
-                    f = exp2_int(e);
+                    uint32_t h[4], l[4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[b][i] *= down;
-                }
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    h[i] = pack_f16(x[b][2 * i], x[b][2 * i + 1]);
-                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-                    l[i] = pack_f16(x[b][2 * i] - y.x, x[b][2 * i + 1] - y.y);
-                }
-                const int at = r * 128 + ((c16 ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                if constexpr (kSplit) {
+                    for (int i = 0; i < 4; ++i) {
+                        const float x0 = x[2 * i] * down, x1 = x[2 * i + 1] * down;
+                        h[i] = pack_f16(x0, x1);
+                        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+                        l[i] = pack_f16(x0 - y.x, x1 - y.y);
+                    }
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[kSplit][g]) + at) = make_uint4(l[0], l[1], l[2], l[3]);
-                    if (col == 0) sm.row_up[r] = f;
+                    if (col == 0) sm.row_up[r] = exp2_int(e);
                 }
             }
         }
@@ -1227,67 +1244,134 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
     if (warp == kSW + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Joins the splits' parts of one row per CTA, in split order: HD / 4 lanes of 4 elements, the other threads
-// take every kPar-th split; their sums meet in shared memory.
+// Joins the splits' parts: the sums weighted by 2^(m - largest m), always in split order.
+template <typename T, int HD, int N>
+__device__ __forceinline__ void join_store(const KvAttnArgs& a, int64_t row, int col, const float (&x)[N], float norm) {
+    const int qh = a.G * a.kv_heads, t = (int)(row / qh), hq = (int)(row - (int64_t)t * qh);
+    T* const p = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) store_out2(p + i, x[i] * norm, x[i + 1] * norm);
+}
+__device__ __forceinline__ float join_lse(float top, float sum) {
+    return sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Few splits (at most kJoinFew): a warp per row, all its parts in flight.
+constexpr int kJoinFew = 8;
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv_attn_join_rows_kernel(const KvAttnArgs a) {
+    pdl_begin();
+    constexpr int kV = HD / 32;  // consecutive elements per lane
+    const int lane = threadIdx.x & 31;
+    const int64_t nrows = (int64_t)a.T * a.G * a.kv_heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= nrows) return;
+    float2 ml[kJoinFew];
+    float y[kJoinFew][kV];
+#pragma unroll
+    for (int s = 0; s < kJoinFew; ++s) {
+        ml[s] = make_float2(-INFINITY, 0.f);
+        if (s < a.splits) {
+            ml[s] = __ldg(a.part_ml + s * nrows + row);
+            const float* const p = a.part_o + (s * nrows + row) * HD + lane * kV;
+            if constexpr (kV == 2) {
+                const float2 u = __ldg(reinterpret_cast<const float2*>(p));
+                y[s][0] = u.x;
+                y[s][1] = u.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kV; i += 4) {
+                    const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+                    y[s][i] = u.x;
+                    y[s][i + 1] = u.y;
+                    y[s][i + 2] = u.z;
+                    y[s][i + 3] = u.w;
+                }
+            }
+        }
+    }
+    float top = -INFINITY, sum = 0.f, x[kV] = {};
+#pragma unroll
+    for (int s = 0; s < kJoinFew; ++s) top = fmaxf(top, ml[s].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int s = 0; s < kJoinFew; ++s) {
+        const float f = ex2_approx(ml[s].x - ref);
+        if (s < a.splits && f != 0.f) {
+            sum = fmaf(ml[s].y, f, sum);
+#pragma unroll
+            for (int i = 0; i < kV; ++i) x[i] = fmaf(y[s][i], f, x[i]);
+        }
+    }
+    join_store<T, HD, kV>(a, row, lane * kV, x, sum == 0.f ? 0.f : 1.f / sum);
+    if (lane == 0 && a.lse != nullptr) a.lse[row] = join_lse(top, sum);
+}
+
+// Many splits of few rows (decode): a CTA per row and 64 columns; 16 threads take each column quad, every 16th
+// split each, and meet in shared memory.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
     pdl_begin();
-    constexpr int kLanes = HD / 4, kPar = 256 / kLanes;
-    __shared__ float w[1024];
-    __shared__ __align__(16) float4 part[kPar][kLanes];
-    __shared__ float red[2];
-    const int tid = threadIdx.x;
-    const int qh = a.G * a.kv_heads;
-    const int64_t row = blockIdx.x, nrows = (int64_t)a.T * qh;
-    if (tid < 32) {
-        float top = -INFINITY, sum = 0.f;
-        for (int s = tid; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[s * nrows + row].x);
+    constexpr int kMost = 320;  // splits, two per thread at most
+    __shared__ float w[kMost], red[2][8];
+    __shared__ __align__(16) float4 part[16][17];
+    const int tid = threadIdx.x, lane = tid & 31, c = tid & 15, s0 = tid >> 4;
+    const int64_t row = blockIdx.x, nrows = (int64_t)a.T * a.G * a.kv_heads;
+    const float* const p = a.part_o + row * HD + blockIdx.y * 64 + c * 4;
+    float2 ml[2];
+    float top = -INFINITY;
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float ref = top == -INFINITY ? 0.f : top;
-        for (int s = tid; s < a.splits; s += 32) {
-            const float2 ml = a.part_ml[s * nrows + row];
-            const float f = ex2_approx(ml.x - ref);
-            w[s] = f;
-            sum += ml.y * f;
-        }
-        sum = group_sum<32>(sum);
-        if (tid == 0) {
-            red[0] = top;
-            red[1] = sum;
-        }
+    for (int i = 0; i < 2; ++i) {
+        const int s = tid + 256 * i;
+        ml[i] = s < a.splits ? __ldg(a.part_ml + s * nrows + row) : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[i].x);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[0][tid >> 5] = top;
     __syncthreads();
-    const float top = red[0], sum = red[1];
-    const int c = tid % kLanes, s0 = tid / kLanes;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[0][i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float f = ex2_approx(ml[i].x - ref);
+        if (tid + 256 * i < a.splits) w[tid + 256 * i] = f;
+        sum = fmaf(ml[i].y, f, sum);
+    }
+    sum = group_sum<32>(sum);
+    if (lane == 0) red[1][tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[1][i];
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = s0; s < a.splits; s += kPar) {
+#pragma unroll 10
+    for (int s = s0; s < a.splits; s += 16) {
         const float f = w[s];
-        if (f == 0.f) continue;
-        const float4 y = *reinterpret_cast<const float4*>(a.part_o + (s * nrows + row) * HD + 4 * c);
-        x.x = fmaf(y.x, f, x.x);
-        x.y = fmaf(y.y, f, x.y);
-        x.z = fmaf(y.z, f, x.z);
-        x.w = fmaf(y.w, f, x.w);
+        const float4 y = __ldg(reinterpret_cast<const float4*>(p + s * nrows * HD));
+        if (f != 0.f) {
+            x.x = fmaf(y.x, f, x.x);
+            x.y = fmaf(y.y, f, x.y);
+            x.z = fmaf(y.z, f, x.z);
+            x.w = fmaf(y.w, f, x.w);
+        }
     }
     part[s0][c] = x;
     __syncthreads();
-    if (s0 != 0) return;
+    if (tid < 16) {
+        float z[4] = {};
 #pragma unroll
-    for (int i = 1; i < kPar; ++i) {
-        const float4 y = part[i][c];
-        x.x += y.x;
-        x.y += y.y;
-        x.z += y.z;
-        x.w += y.w;
+        for (int i = 0; i < 16; ++i) {
+            const float4 y = part[i][tid];
+            z[0] += y.x;
+            z[1] += y.y;
+            z[2] += y.z;
+            z[3] += y.w;
+        }
+        join_store<T, HD, 4>(a, row, blockIdx.y * 64 + tid * 4, z, sum == 0.f ? 0.f : 1.f / sum);
+        if (tid == 0 && blockIdx.y == 0 && a.lse != nullptr) a.lse[row] = join_lse(top, sum);
     }
-    const float norm = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = (int)(row / qh), hq = (int)(row % qh);
-    T* const p = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + 4 * c;
-    store_out2(p, x.x * norm, x.y * norm);
-    store_out2(p + 2, x.z * norm, x.w * norm);
-    if (tid == 0 && a.lse != nullptr) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Which kernel a call takes and how far the keys may be split, from the sizes alone (the key count is only
@@ -1321,7 +1405,11 @@ static int launch_attn(KvAttnArgs& a, const AttnShape& s, cudaStream_t stream) {
         if (rc != WZYB_OK) return rc;
         launch_k(kern, grid, TcSmem<T, HD>::kThreads, smem, stream, a);
     }
-    if (a.splits > 1) launch_k(kv_attn_join_kernel<T, HD>, a.T * a.G * a.kv_heads, 256, 0, stream, a);
+    const int out_rows = a.T * a.G * a.kv_heads;
+    if (a.splits > kJoinFew)
+        launch_k(kv_attn_join_kernel<T, HD>, dim3(out_rows, HD / 64), 256, 0, stream, a);
+    else if (a.splits > 1)
+        launch_k(kv_attn_join_rows_kernel<T, HD>, (out_rows + 7) / 8, 256, 0, stream, a);
     return launch_status();
 }
 
