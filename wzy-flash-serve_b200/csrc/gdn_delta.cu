@@ -617,11 +617,13 @@ __device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
 // 8 value columns of a head belong to two warps from the first chunk to the last. The state warp keeps its part of S
 // in its registers as fp32 accumulator tiles; S, X = V - e^G K S and d = T X pass from product to product inside it
 // (columns never mix), so its chain, which is what the chunks wait for, needs no barrier but the one per chunk. The
-// output warp takes S and d from it as operands and makes o = e^G Q S + P d meanwhile (one warp for both
-// took 1.5 times as long: the chain leaves most issue slots empty). The CTA's four pairs share the chunk's K, Q, T
-// and P in shared memory, fetched by cp.async while the chunk before is worked through.
+// output warp takes S and d from it as operands and makes o = e^G Q S + P d in the time in which the
+// state warp has few products to do (it starts when K S is done: the two products at once share the tensor pipe and
+// the chain waits). The CTA's four pairs share the chunk's K, Q, T and P in shared memory; four more warps fetch the
+// next chunk's by cp.async (done by the state warps it cost their chain 1300 cycles of 5800 per chunk; bulk copies
+// of 256-byte rows by one warp took 7000).
 template <typename T, int HD>
-__global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
+__global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
     pdl_begin();
     using Stage = GdnScanStage<T, HD>;
     constexpr bool kSplit = Stage::kSplit;
@@ -630,68 +632,73 @@ __global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArg
     Stage* const st = reinterpret_cast<Stage*>(smem_raw);
     const GdnDeltaArgs& a = p.x;
     const int tid = threadIdx.x, lane = tid & 31, pair = (tid >> 5) & 3, g = lane >> 2, t4 = lane & 3;
-    const bool out_warp = tid >= 128;
+    const int role = tid >> 7;  // 0 state, 1 output, 2 fetch
     GdnHandOver<HD>& hand = reinterpret_cast<GdnHandOver<HD>*>(smem_raw + 2 * sizeof(Stage))[pair];
     const int h = blockIdx.x / (HD / 32), c0 = (blockIdx.x % (HD / 32)) * 32;
     const int hk = h / (a.v_heads / a.k_heads);
     const int chunks = (int)((p.t1 - p.t0 + kGdnChunk - 1) / kGdnChunk);
 
-    auto fetch = [&](int ch) {
-        Stage& s = st[ch & 1];
-        const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
-        const int n = (int)(p.t1 - tok0 < kGdnChunk ? p.t1 - tok0 : kGdnChunk);
-        constexpr int kRowChunks = HD / 8;
-        if constexpr (kSplit) {
-            const __half* const src = p.kq + ((int64_t)ch * a.k_heads + hk) * (4 * 64 * HD);
-#pragma unroll 4
-            for (int i = tid; i < 4 * 64 * kRowChunks; i += 256) {
-                const int m = i / (64 * kRowChunks), r = (i / kRowChunks) % 64, c = (i % kRowChunks) * 8;
-                __half* const base = m < 2 ? s.k[m & 1] : s.q[m & 1];
-                cp_async16(base + r * kLd + c, src + (m * 64 + r) * HD + c);
+    if (role == 2) {
+        const int u = tid & 127;
+        for (int ch = 0; ch <= chunks; ++ch) {  // chunk ch is fetched while ch - 1 is worked through
+            if (ch > 0) {
+                cp_async_wait<0>();
+                __syncthreads();  // chunk ch - 1 is there for all, and nobody reads chunk ch - 2's buffers any more
             }
-        } else {
-            // a thread keeps its piece of the row; rows go up by 256 / pieces
-            const int c = (tid % kRowChunks) * 8, r0 = tid / kRowChunks;
-            constexpr int kStep = 256 / kRowChunks;
+            if (ch == chunks) break;
+            Stage& s = st[ch & 1];
+            const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
+            const int n = (int)(p.t1 - tok0 < kGdnChunk ? p.t1 - tok0 : kGdnChunk);
+            constexpr int kPieces = HD / 8;
+            const int c = (u % kPieces) * 8, r0 = u / kPieces;  // a thread keeps its piece of the row
+            constexpr int kStep = 128 / kPieces;
+            if constexpr (kSplit) {
+                const __half* src = p.kq + ((int64_t)ch * a.k_heads + hk) * (4 * 64 * HD) + r0 * HD + c;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int64_t row = m ? a.q_row : a.k_row;
-                const __half* src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r0) * row + hk * HD + c;
-                __half* dst = (m ? s.q[0] : s.k[0]) + r0 * kLd + c;
+                for (int m = 0; m < 4; ++m) {
+                    __half* dst = (m < 2 ? s.k[m & 1] : s.q[m & 1]) + r0 * kLd + c;
 #pragma unroll
-                for (int r = r0; r < 64; r += kStep, src += kStep * row, dst += kStep * kLd) {
-                    if (r < n)
-                        cp_async16(dst, src);
-                    else
-                        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+                    for (int r = 0; r < 64; r += kStep, src += kStep * HD, dst += kStep * kLd) cp_async16(dst, src);
+                }
+            } else {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const int64_t row = m ? a.q_row : a.k_row;
+                    const __half* src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r0) * row + hk * HD + c;
+                    __half* dst = (m ? s.q[0] : s.k[0]) + r0 * kLd + c;
+#pragma unroll
+                    for (int r = r0; r < 64; r += kStep, src += kStep * row, dst += kStep * kLd) {
+                        if (r < n)
+                            cp_async16(dst, src);
+                        else
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+                    }
                 }
             }
-        }
-        constexpr int kVC = 32 * sizeof(T) / 16, kVE = 16 / sizeof(T);
+            constexpr int kVC = 32 * sizeof(T) / 16, kVE = 16 / sizeof(T);
 #pragma unroll
-        for (int i = tid; i < 64 * kVC; i += 256) {
-            const int r = i / kVC, c = (i % kVC) * kVE;
-            T* const dst = s.v + r * kVLd + c;
-            if (r < n)
-                cp_async16(dst, static_cast<const T*>(a.v) + (tok0 + r) * a.v_row + h * HD + c0 + c);
-            else
-                *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-        }
-        const uint4* const src = reinterpret_cast<const uint4*>(p.data + ((int64_t)ch * a.v_heads + h) * sizeof(GdnChunkData<kSplit>));
-        uint4* const dst = reinterpret_cast<uint4*>(&s.d);
+            for (int i = u; i < 64 * kVC; i += 128) {
+                const int r = i / kVC, cv = (i % kVC) * kVE;
+                T* const dst = s.v + r * kVLd + cv;
+                if (r < n)
+                    cp_async16(dst, static_cast<const T*>(a.v) + (tok0 + r) * a.v_row + h * HD + c0 + cv);
+                else
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            }
+            const uint4* const src = reinterpret_cast<const uint4*>(p.data + ((int64_t)ch * a.v_heads + h) * sizeof(GdnChunkData<kSplit>));
+            uint4* const dst = reinterpret_cast<uint4*>(&s.d);
 #pragma unroll
-        for (int i = tid; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 256) cp_async16(dst + i, src + i);
-        cp_async_commit();
-    };
+            for (int i = u; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 128) cp_async16(dst + i, src + i);
+            cp_async_commit();
+        }
+        return;
+    }
 
     const int col = c0 + pair * 8 + 2 * t4;  // this lane's columns col, col + 1
     const int arow = lane & 15, acol = (lane >> 4) * 8;
-    fetch(0);
-    if (out_warp) {
+    if (role == 1) {
         for (int ch = 0; ch < chunks; ++ch) {
-            cp_async_wait<0>();
-            __syncthreads();  // chunk ch is there for all, and nobody still reads the other buffers
-            if (ch + 1 < chunks) fetch(ch + 1);
+            __syncthreads();  // chunk ch is there; chunk ch - 1's buffers, and what the pair handed over, are free
             const Stage& z = st[ch & 1];
             named_bar_sync(1 + pair, 64);  // S
             uint4 so[kM];
@@ -761,9 +768,7 @@ __global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArg
             s[i][c] = p.state_in != nullptr ? sin[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] : 0.f;
     int es[2] = {0, 0}, ex[2] = {0, 0}, ed[2] = {0, 0}, ec[2] = {0, 0};
     for (int ch = 0; ch < chunks; ++ch) {
-        cp_async_wait<0>();
         __syncthreads();
-        if (ch + 1 < chunks) fetch(ch + 1);
         const Stage& z = st[ch & 1];
         const bool force = (ch & 15) == 0;
 
@@ -773,7 +778,6 @@ __global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArg
         const float su[2] = {gdn_exp2i(es[0]), gdn_exp2i(es[1])};
         gdn_hand(hand.s, sh, sl, lane);
         hand.s_up[lane] = make_float2(su[0], su[1]);
-        named_bar_arrive(1 + pair, 64);
         float x[4][4];
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {  // two row tiles at a time: four independent chains of products
@@ -800,6 +804,7 @@ __global__ void __launch_bounds__(256, 1) gdn_chunk_scan_kernel(const GdnScanArg
                     x[i + j][c] = v - z.d.a[r] * su[c & 1] * fmaf(kl[j][c], 1.f / kGdnLo, kh[j][c]);
                 }
         }
+        named_bar_arrive(1 + pair, 64);
         // d = T X
         uint32_t xh[4][2], xl[4][2];
         gdn_col_exp(x, ex, force);
@@ -903,7 +908,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
         sa.t1 = t1;
         const int64_t chunks = (t1 - t0 + kGdnChunk - 1) / kGdnChunk;
         launch_k(prep, (unsigned)(chunks * a.k_heads), 128, prep_smem, stream, pa);
-        launch_k(scan, a.v_heads * (HD / 32), 256, scan_smem, stream, sa);
+        launch_k(scan, a.v_heads * (HD / 32), 384, scan_smem, stream, sa);
         sa.state_in = a.state_out;
     }
     return launch_status();
