@@ -735,10 +735,20 @@ struct TcSmem {
     int e_key[2][kN], e_max[2][2];
     int4 tile[2];  // position, keys, kTile* flags
     int bad[2][2];
+    // one warp's 32 rows of kOutCols columns on their way out; for HD = 256 they take the operands' place
+    static constexpr int kOutCols = HD / kParts < 32 ? HD / kParts : 32, kOutLd = kOutCols + 4, kOutWarp = 32 * kOutLd;
+    float out[HD == 256 ? 4 : kSW * kOutWarp];
     uint64_t k_full, v_full, s_full[kPairs], p_full[kPairs], x_full[4], o_full, done;
     KeyPlan plan;
     uint32_t tmem;
 };
+
+// Element offset of query row `row` of a kv head, -1 past the last one.
+__device__ __forceinline__ int64_t q_offset(const KvAttnArgs& a, int head, int row, int rows) {
+    if (row >= rows) return -1;
+    const int t = row / a.G;
+    return t * a.q_row + (int64_t)(head * a.G + (row - t * a.G)) * a.q_head;
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
@@ -771,26 +781,23 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
         fence_mbar_init();
     }
     if (warp < kSW) {
-        // Query rows to shared memory, a lane 8 elements, all of a warp's rows in flight (two turns for fp32). fp32
+        // Query rows to shared memory, a lane 8 elements, several rows of a warp in flight. fp32
         // rows enter as two fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range.
-        constexpr int kL = HD / 8, kPer = 32 / kL, kMineQ = S::kRows / kSW / kPer;  // lanes per row, rows at a time, loads
-        constexpr int kBatch = kMineQ < 8 ? kMineQ : 8;
+        constexpr int kL = HD / 8, kPer = 32 / kL, kRowsQ = S::kRows / kSW, kMineQ = kRowsQ / kPer;  // lanes per row, rows
+        constexpr int kMostQ = kSplit ? 4 : 8, kBatch = kMineQ < kMostQ ? kMineQ : kMostQ;          // at a time, ...
         const int col = (lane % kL) * 8, g = col / 64, c16 = (col % 64) / 8;
+        // lane i finds the warp's row i (one division per warp: straight code that runs once costs its fetch)
+        const int64_t mine_at = q_offset(a, head, row0 + warp * kRowsQ + lane % kRowsQ, rows);
 #pragma unroll 1
-        for (int r0 = warp * kPer * kMineQ; r0 < (warp + 1) * kPer * kMineQ; r0 += kPer * kBatch) {
+        for (int r0 = warp * kRowsQ; r0 < (warp + 1) * kRowsQ; r0 += kPer * kBatch) {
             uint4 raw[kBatch][sizeof(T) / 2];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                const int row = row0 + r0 + b * kPer + lane / kL;
+                const int64_t at = __shfl_sync(0xffffffffu, mine_at, r0 - warp * kRowsQ + b * kPer + lane / kL);
 #pragma unroll
-                for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[b][i] = make_uint4(0, 0, 0, 0);
-                if (row < rows) {
-                    const int t = row / a.G, gq = row - t * a.G;
-                    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + t * a.q_row +
-                                                                          (int64_t)(head * a.G + gq) * a.q_head + col);
-#pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[b][i] = __ldg(p + i);
-                }
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                    raw[b][i] = at < 0 ? make_uint4(0, 0, 0, 0)
+                                       : __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at + col) + i);
             }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
@@ -1055,35 +1062,50 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
                 else if (a.lse != nullptr)
                     a.lse[orow] = l == 0.f ? -INFINITY : (m + (float)(unit(E) - 7) + log2f(l)) * 0.6931471805599453f;
             }
-            T* const po = static_cast<T*>(a.out) + t * a.o_row + hq * a.o_head + part * kDims;
-            float* const pp = a.part_o + at * HD + part * kDims;
+            // Through shared memory, so that a row's columns leave as whole 128-byte lines (a lane's own row, 16
+            // bytes at a time, took 5 us for 128 rows of 256).
+            constexpr int kCols = S::kOutCols, kLd = S::kOutLd, kQuads = kCols / 4, kRowsAt = 32 / kQuads;
+            static_assert(HD < 256 || kSW * S::kOutWarp * 4 <= (int)(sizeof(sm.q) + sizeof(sm.k) + sizeof(sm.v)), "the operands' place");
+            float* const slab = (HD == 256 ? reinterpret_cast<float*>(&sm.q) : sm.out) + warp * S::kOutWarp;
+            // element offset of this lane's row in the output or the parts, -1 past the last row
+            const int64_t my_at = row >= rows ? -1 : (a.splits > 1 ? at * HD : t * a.o_row + hq * a.o_head) + part * kDims;
 #pragma unroll
-            for (int c = 0; c < kDims; c += 16) {
-                float x[16];
-                if constexpr (kSplit) {
+            for (int c = 0; c < kDims; c += kCols) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = o[c + i] * norm;
-                } else if (te > tb) {
-                    tc_ld16(x, o_at + c);
-                    tc_wait_ld();
+                for (int i = 0; i < kCols; i += 16) {
+                    float x[16];
+                    if constexpr (kSplit) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = l == 0.f ? 0.f : x[i] * norm;
-                } else {
+                        for (int j = 0; j < 16; ++j) x[j] = o[c + i + j] * norm;
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+                        for (int j = 0; j < 16; ++j) x[j] = 0.f;
+                        if (te > tb) {
+                            tc_ld16(x, o_at + c + i);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[j] = l == 0.f ? 0.f : x[j] * norm;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        *reinterpret_cast<float4*>(slab + lane * kLd + i + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                 }
-                if (row >= rows) continue;
-                if (a.splits > 1 || kSplit) {
-                    float* const d = a.splits > 1 ? pp : reinterpret_cast<float*>(po);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4*>(d + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 8)
-                        *reinterpret_cast<uint4*>(po + c + i) = make_uint4(pack_f16(x[i], x[i + 1]), pack_f16(x[i + 2], x[i + 3]),
-                                                                           pack_f16(x[i + 4], x[i + 5]), pack_f16(x[i + 6], x[i + 7]));
+                __syncwarp();
+                const int cq = (lane % kQuads) * 4;
+#pragma unroll 1
+                for (int i = lane / kQuads; i < 32; i += kRowsAt) {
+                    const float4 y = *reinterpret_cast<const float4*>(slab + i * kLd + cq);
+                    const int64_t to = __shfl_sync(0xffffffffu, my_at, i) + c + cq;
+                    if (to < c + cq) continue;
+                    if (a.splits > 1) {
+                        *reinterpret_cast<float4*>(a.part_o + to) = y;
+                    } else {
+                        store_out2(static_cast<T*>(a.out) + to, y.x, y.y);
+                        store_out2(static_cast<T*>(a.out) + to + 2, y.z, y.w);
+                    }
                 }
+                __syncwarp();
             }
         }
     } else if (warp < kSW + 4) {
