@@ -235,18 +235,27 @@ __device__ __forceinline__ int gdn_exp(float x) {
 }
 __device__ __forceinline__ float gdn_exp2i(int e) { return __int_as_float((e + 127) << 23); }
 
+// A (chunk, k head)'s K and Q as the scan's shared memory holds them (rows padded by 16 bytes, missing tokens zero), so
+// that one bulk copy fetches them: 64 rows by cp.async took the scan's load/store unit 450 cycles per chunk, and
+// a bulk copy per row far longer. fp32 inputs as two fp16 parts each.
+template <bool kSplit, int HD>
+struct GdnKq {
+    static constexpr int kLd = HD + 8;
+    __half k[kSplit ? 2 : 1][64 * kLd], q[kSplit ? 2 : 1][64 * kLd];
+};
+
 struct GdnPrepArgs {
     GdnDeltaArgs x;
-    int64_t t0;      // first token of the segment
-    uint8_t* data;   // [chunks, v_heads] GdnChunkData
-    __half* kq;      // fp32 calls: [chunks, k_heads, 4 (k hi, k lo, q hi, q lo), 64, HD]
+    int64_t t0;     // first token of the segment
+    uint8_t* data;  // [chunks, v_heads] GdnChunkData
+    uint8_t* kq;    // [chunks, k_heads] GdnKq
 };
 
 template <typename T, int HD>
 struct GdnPrepSmem {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kLd = HD + 8;
-    __half k[kSplit ? 2 : 1][64 * kLd], q[kSplit ? 2 : 1][64 * kLd];
+    GdnKq<kSplit, HD> kq;
     float A[64][68];
     float tm[64][68];
     float rk[64], rq[64], beta[64], ghi[64], glo[64];
@@ -270,6 +279,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
     const int64_t tok0 = p.t0 + (int64_t)chunk * kGdnChunk;
     const int n = (int)(a.T - tok0 < kGdnChunk ? a.T - tok0 : kGdnChunk);
     constexpr int kL = HD / 8;  // lanes per row
+    GdnKq<kSplit, HD>& image = reinterpret_cast<GdnKq<kSplit, HD>*>(p.kq)[(int64_t)chunk * a.k_heads + hk];
 
     for (int r0 = 0; r0 < 64; r0 += 128 / kL) {
         const int r = r0 + tid / kL, col = (tid % kL) * 8;
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             }
             ss = group_sum<kL>(ss);
             f[m] = r < n ? (a.l2norm ? rsqrtf(ss + a.l2_eps) : 1.f) : 0.f;
-            __half* const hi = (m ? sm.q[0] : sm.k[0]) + r * kLd + col;
+            __half* const hi = (m ? sm.kq.q[0] : sm.kq.k[0]) + r * kLd + col;
             if constexpr (kSplit) {
 #pragma unroll
                 for (int o = kL / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
@@ -304,12 +314,13 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
                 for (int i = 0; i < 4; ++i) gdn_split(x[m][2 * i] * down, x[m][2 * i + 1] * down, h[i], l[i]);
                 const uint4 vh = make_uint4(h[0], h[1], h[2], h[3]), vl = make_uint4(l[0], l[1], l[2], l[3]);
                 *reinterpret_cast<uint4*>(hi) = vh;
-                *reinterpret_cast<uint4*>((m ? sm.q[kSplit] : sm.k[kSplit]) + r * kLd + col) = vl;
-                __half* const dst = p.kq + ((int64_t)chunk * a.k_heads + hk) * (4 * 64 * HD) + m * (2 * 64 * HD) + r * HD + col;
-                *reinterpret_cast<uint4*>(dst) = vh;
-                *reinterpret_cast<uint4*>(dst + 64 * HD) = vl;
+                *reinterpret_cast<uint4*>((m ? sm.kq.q[kSplit] : sm.kq.k[kSplit]) + r * kLd + col) = vl;
+                *reinterpret_cast<uint4*>((m ? image.q[0] : image.k[0]) + r * kLd + col) = vh;
+                *reinterpret_cast<uint4*>((m ? image.q[kSplit] : image.k[kSplit]) + r * kLd + col) = vl;
             } else {
-                *reinterpret_cast<uint4*>(hi) = Vec8<__half>::from_f32(x[m]);
+                const uint4 v = Vec8<__half>::from_f32(x[m]);
+                *reinterpret_cast<uint4*>(hi) = v;
+                *reinterpret_cast<uint4*>((m ? image.q[0] : image.k[0]) + r * kLd + col) = v;
             }
         }
         if (col == 0) {
@@ -324,8 +335,8 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         float (&acc)[8][4] = m ? qk : kk;
-        const __half* const xh = m ? sm.q[0] : sm.k[0];
-        const __half* const xl = m ? sm.q[kSplit] : sm.k[kSplit];
+        const __half* const xh = m ? sm.kq.q[0] : sm.kq.k[0];
+        const __half* const xl = m ? sm.kq.q[kSplit] : sm.kq.k[kSplit];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -344,11 +355,11 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
                     if (i > warp) break;  // warp-uniform
                     uint32_t fb[4];
                     if (part == 1) {
-                        ldmatrix_x4(fb, sm.k[kSplit] + (i * 16 + brow) * kLd + ks * 16 + bcol);
+                        ldmatrix_x4(fb, sm.kq.k[kSplit] + (i * 16 + brow) * kLd + ks * 16 + bcol);
                         mma_f16(acc[2 * i], fa, fb[0], fb[1]);
                         mma_f16(acc[2 * i + 1], fa, fb[2], fb[3]);
                     }
-                    ldmatrix_x4(fb, sm.k[0] + (i * 16 + brow) * kLd + ks * 16 + bcol);
+                    ldmatrix_x4(fb, sm.kq.k[0] + (i * 16 + brow) * kLd + ks * 16 + bcol);
                     if (part == 1) {
                         mma_f16(acc[2 * i], fl, fb[0], fb[1]);
                         mma_f16(acc[2 * i + 1], fl, fb[2], fb[3]);
@@ -368,6 +379,16 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
     }
 
     const int per = a.v_heads / a.k_heads;
+    float gx[2] = {0.f, 0.f}, bx[2] = {0.f, 0.f};  // warp 0: g and beta of tokens 2 * lane, + 1, a head ahead
+    auto load_gb = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (2 * lane + i < n) {
+                gx[i] = __ldg(a.g + (tok0 + 2 * lane + i) * a.v_heads + h);
+                bx[i] = __ldg(a.beta + (tok0 + 2 * lane + i) * a.v_heads + h);
+            }
+    };
+    if (warp == 0) load_gb(hk * per);
     for (int hv = 0; hv < per; ++hv) {
         const int h = hk * per + hv;
         GdnChunkData<kSplit>& out =
@@ -378,16 +399,10 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             double s0 = 0., s1 = 0.;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int t = 2 * lane + i;
-                float x = 0.f, b = 0.f;
-                if (t < n) {
-                    x = a.g[(tok0 + t) * a.v_heads + h];
-                    b = a.beta[(tok0 + t) * a.v_heads + h];
-                    x = x < -120.f ? -120.f : x;
-                }
-                sm.beta[t] = b;
-                (i ? s1 : s0) = (double)x * 1.4426950408889634;
+                sm.beta[2 * lane + i] = bx[i];
+                (i ? s1 : s0) = (double)(gx[i] < -120.f ? -120.f : gx[i]) * 1.4426950408889634;
             }
+            if (hv + 1 < per) load_gb(h + 1);
             s1 += s0;
             double run = s1;
 #pragma unroll
@@ -544,16 +559,16 @@ struct GdnScanArgs {
     int64_t t0, t1;  // the segment's tokens
     const float* state_in;
     const uint8_t* data;
-    const __half* kq;
+    const uint8_t* kq;
 };
 
 template <typename T, int HD>
 struct GdnScanStage {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kLd = HD + 8, kVLd = 32 + 16 / sizeof(T);
-    __half k[kSplit ? 2 : 1][64 * kLd], q[kSplit ? 2 : 1][64 * kLd];
-    T v[64 * kVLd];
+    GdnKq<kSplit, HD> kq;
     GdnChunkData<kSplit> d;
+    T v[64 * kVLd];
 };
 
 // Two column exponents per lane (columns 2*t4, 2*t4 + 1 of its warp), alike over the lanes of a column: values
@@ -597,13 +612,14 @@ __device__ __forceinline__ void gdn_operand(const float (&x)[N][4], const int (&
         }
 }
 
-// What a state warp hands to its output warp, as second operands (16 bytes per lane and index): S at the chunk's
-// start and d, each with the scales of its two columns per lane.
+// What a state warp hands to its output warp: S at the chunk's start as a second operand (per step of 16: hi, hi,
+// lo, lo) with the scales of a lane's two columns, and d as fp32 accumulator tiles (the output warp has the time to
+// make an operand of it, the state warp's chain has not).
 template <int HD>
 struct GdnHandOver {
-    uint4 s[HD / 16][32];  // per step of 16: hi, hi, lo, lo
-    uint4 d[4][32];
-    float2 s_up[32], d_up[32];
+    uint4 s[HD / 16][32];
+    float4 d[4][32];
+    float2 s_up[32];
 };
 template <int N>
 __device__ __forceinline__ void gdn_hand(uint4 (&to)[N][32], const uint32_t (&hi)[N][2], const uint32_t (&lo)[N][2], int lane) {
@@ -617,13 +633,11 @@ __device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
 // 8 value columns of a head belong to two warps from the first chunk to the last. The state warp keeps its part of S
 // in its registers as fp32 accumulator tiles; S, X = V - e^G K S and d = T X pass from product to product inside it
 // (columns never mix), so its chain, which is what the chunks wait for, needs no barrier but the one per chunk. The
-// output warp takes S and d from it as operands and makes o = e^G Q S + P d in the time in which the
-// state warp has few products to do (it starts when K S is done: the two products at once share the tensor pipe and
-// the chain waits). The CTA's four pairs share the chunk's K, Q, T and P in shared memory; four more warps fetch the
-// next chunk's by cp.async (done by the state warps it cost their chain 1300 cycles of 5800 per chunk; bulk copies
-// of 256-byte rows by one warp took 7000).
+// output warp takes S and d from it when T X is done and makes o = e^G Q S + P d beside the rest of the chunk and the
+// start of the next one (one warp for both took 1.5 times as long). The CTA's four pairs share the chunk's K, Q, T and P in shared memory; a ninth warp fetches the
+// next chunk's meanwhile.
 template <typename T, int HD>
-__global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
+__global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
     pdl_begin();
     using Stage = GdnScanStage<T, HD>;
     constexpr bool kSplit = Stage::kSplit;
@@ -638,46 +652,41 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
     const int hk = h / (a.v_heads / a.k_heads);
     const int chunks = (int)((p.t1 - p.t0 + kGdnChunk - 1) / kGdnChunk);
 
+    uint64_t* const full = reinterpret_cast<uint64_t*>(smem_raw + 2 * sizeof(Stage) + 4 * sizeof(GdnHandOver<HD>) + 16);
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+
+    // named barriers: chunk ready (fetch, state), buffers free (fetch, output), handed over and taken (each pair)
+    constexpr int kBarReady = 1, kBarFree = 2, kBarHand = 3, kBarTaken = 7;
     if (role == 2) {
-        const int u = tid & 127;
+        const uint64_t policy = policy_evict_normal();
+        bool ok = true;  // a wait for a chunk that gave up is not repeated
         for (int ch = 0; ch <= chunks; ++ch) {  // chunk ch is fetched while ch - 1 is worked through
             if (ch > 0) {
                 cp_async_wait<0>();
-                __syncthreads();  // chunk ch - 1 is there for all, and nobody reads chunk ch - 2's buffers any more
+                ok = ok && mbar_wait(&full[(ch - 1) & 1], ((ch - 1) >> 1) & 1);
+                named_bar_sync(kBarReady, 160);  // chunk ch - 1 is there for the state warps
+                // the output warps have begun chunk ch - 1, so nobody reads chunk ch - 2's buffers any more; the state
+                // warps are past the products that the copies would slow down
+                named_bar_sync(kBarFree, 160);
             }
             if (ch == chunks) break;
             Stage& s = st[ch & 1];
+            if (lane == 0) {
+                constexpr int kKq = sizeof(GdnKq<kSplit, HD>), kData = sizeof(GdnChunkData<kSplit>);
+                mbar_arrive_expect_tx(&full[ch & 1], kKq + kData);
+                bulk_load(&s.kq, p.kq + ((int64_t)ch * a.k_heads + hk) * kKq, kKq, &full[ch & 1], policy);
+                bulk_load(&s.d, p.data + ((int64_t)ch * a.v_heads + h) * kData, kData, &full[ch & 1], policy);
+            }
             const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
             const int n = (int)(p.t1 - tok0 < kGdnChunk ? p.t1 - tok0 : kGdnChunk);
-            constexpr int kPieces = HD / 8;
-            const int c = (u % kPieces) * 8, r0 = u / kPieces;  // a thread keeps its piece of the row
-            constexpr int kStep = 128 / kPieces;
-            if constexpr (kSplit) {
-                const __half* src = p.kq + ((int64_t)ch * a.k_heads + hk) * (4 * 64 * HD) + r0 * HD + c;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    __half* dst = (m < 2 ? s.k[m & 1] : s.q[m & 1]) + r0 * kLd + c;
-#pragma unroll
-                    for (int r = 0; r < 64; r += kStep, src += kStep * HD, dst += kStep * kLd) cp_async16(dst, src);
-                }
-            } else {
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    const int64_t row = m ? a.q_row : a.k_row;
-                    const __half* src = static_cast<const __half*>(m ? a.q : a.k) + (tok0 + r0) * row + hk * HD + c;
-                    __half* dst = (m ? s.q[0] : s.k[0]) + r0 * kLd + c;
-#pragma unroll
-                    for (int r = r0; r < 64; r += kStep, src += kStep * row, dst += kStep * kLd) {
-                        if (r < n)
-                            cp_async16(dst, src);
-                        else
-                            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-                    }
-                }
-            }
             constexpr int kVC = 32 * sizeof(T) / 16, kVE = 16 / sizeof(T);
-#pragma unroll
-            for (int i = u; i < 64 * kVC; i += 128) {
+#pragma unroll 4
+            for (int i = lane; i < 64 * kVC; i += 32) {
                 const int r = i / kVC, cv = (i % kVC) * kVE;
                 T* const dst = s.v + r * kVLd + cv;
                 if (r < n)
@@ -685,26 +694,32 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
                 else
                     *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
             }
-            const uint4* const src = reinterpret_cast<const uint4*>(p.data + ((int64_t)ch * a.v_heads + h) * sizeof(GdnChunkData<kSplit>));
-            uint4* const dst = reinterpret_cast<uint4*>(&s.d);
-#pragma unroll
-            for (int i = u; i < (int)(sizeof(GdnChunkData<kSplit>) / 16); i += 128) cp_async16(dst + i, src + i);
             cp_async_commit();
         }
         return;
     }
-
     const int col = c0 + pair * 8 + 2 * t4;  // this lane's columns col, col + 1
     const int arow = lane & 15, acol = (lane >> 4) * 8;
     if (role == 1) {
+        int ed[2] = {0, 0};
         for (int ch = 0; ch < chunks; ++ch) {
-            __syncthreads();  // chunk ch is there; chunk ch - 1's buffers, and what the pair handed over, are free
             const Stage& z = st[ch & 1];
-            named_bar_sync(1 + pair, 64);  // S
+            named_bar_sync(kBarHand + pair, 64);  // S and d (and, through the state warp, the chunk's data)
+            named_bar_arrive(kBarFree, 160);
             uint4 so[kM];
+            float d[4][4];
 #pragma unroll
             for (int i = 0; i < kM; ++i) so[i] = hand.s[i][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 y = hand.d[i][lane];
+                d[i][0] = y.x;
+                d[i][1] = y.y;
+                d[i][2] = y.z;
+                d[i][3] = y.w;
+            }
             const float2 su = hand.s_up[lane];
+            named_bar_arrive(kBarTaken + pair, 64);
             float o[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -712,11 +727,11 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
                 for (int ks = 0; ks < kM; ++ks) {
                     uint32_t fq[4];
-                    ldmatrix_x4(fq, z.q[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                    ldmatrix_x4(fq, z.kq.q[0] + (i * 16 + arow) * kLd + ks * 16 + acol);
                     mma_f16(qh, fq, so[ks].x, so[ks].y);
                     mma_f16(ql, fq, so[ks].z, so[ks].w);
                     if constexpr (kSplit) {
-                        ldmatrix_x4(fq, z.q[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
+                        ldmatrix_x4(fq, z.kq.q[kSplit] + (i * 16 + arow) * kLd + ks * 16 + acol);
                         mma_f16(ql, fq, so[ks].x, so[ks].y);
                     }
                 }
@@ -724,12 +739,10 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
                 for (int c = 0; c < 4; ++c)
                     o[i][c] = z.d.b[16 * i + g + (c >> 1) * 8] * (c & 1 ? su.y : su.x) * fmaf(ql[c], 1.f / kGdnLo, qh[c]);
             }
-            named_bar_sync(5 + pair, 64);  // d
-            uint4 dd[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dd[i] = hand.d[i][lane];
-            const float2 du = hand.d_up[lane];
-            const float2 up = make_float2(du.x * z.d.p_up, du.y * z.d.p_up);
+            uint32_t dh[4][2], dl[4][2];
+            gdn_col_exp(d, ed, (ch & 15) == 0);
+            gdn_operand(d, ed, dh, dl);
+            const float2 up = make_float2(gdn_exp2i(ed[0]) * z.d.p_up, gdn_exp2i(ed[1]) * z.d.p_up);
             const int64_t tok0 = p.t0 + (int64_t)ch * kGdnChunk;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -737,9 +750,9 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
                 for (int j = 0; j <= i; ++j) {
                     const uint4 ph = z.d.p[i * (i + 1) / 2 + j][lane];
-                    mma_f16(oh, ph, dd[j].x, dd[j].y);
-                    mma_f16(ol, ph, dd[j].z, dd[j].w);
-                    if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dd[j].x, dd[j].y);
+                    mma_f16(oh, ph, dh[j][0], dh[j][1]);
+                    mma_f16(ol, ph, dl[j][0], dl[j][1]);
+                    if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dh[j][0], dh[j][1]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[i][c] = fmaf(c & 1 ? up.y : up.x, fmaf(ol[c], 1.f / kGdnLo, oh[c]), o[i][c]);
@@ -766,9 +779,9 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             s[i][c] = p.state_in != nullptr ? sin[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] : 0.f;
-    int es[2] = {0, 0}, ex[2] = {0, 0}, ed[2] = {0, 0}, ec[2] = {0, 0};
+    int es[2] = {0, 0}, ex[2] = {0, 0}, ec[2] = {0, 0};
     for (int ch = 0; ch < chunks; ++ch) {
-        __syncthreads();
+        named_bar_sync(kBarReady, 160);
         const Stage& z = st[ch & 1];
         const bool force = (ch & 15) == 0;
 
@@ -776,6 +789,7 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
         gdn_col_exp(s, es, force);
         gdn_operand(s, es, sh, sl);
         const float su[2] = {gdn_exp2i(es[0]), gdn_exp2i(es[1])};
+        if (ch > 0) named_bar_sync(kBarTaken + pair, 64);
         gdn_hand(hand.s, sh, sl, lane);
         hand.s_up[lane] = make_float2(su[0], su[1]);
         float x[4][4];
@@ -787,11 +801,11 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     uint32_t fk[4];
-                    ldmatrix_x4(fk, z.k[0] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
+                    ldmatrix_x4(fk, z.kq.k[0] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
                     mma_f16(kh[j], fk, sh[ks][0], sh[ks][1]);
                     mma_f16(kl[j], fk, sl[ks][0], sl[ks][1]);
                     if constexpr (kSplit) {
-                        ldmatrix_x4(fk, z.k[kSplit] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
+                        ldmatrix_x4(fk, z.kq.k[kSplit] + ((i + j) * 16 + arow) * kLd + ks * 16 + acol);
                         mma_f16(kl[j], fk, sh[ks][0], sh[ks][1]);
                     }
                 }
@@ -804,7 +818,6 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
                     x[i + j][c] = v - z.d.a[r] * su[c & 1] * fmaf(kl[j][c], 1.f / kGdnLo, kh[j][c]);
                 }
         }
-        named_bar_arrive(1 + pair, 64);
         // d = T X
         uint32_t xh[4][2], xl[4][2];
         gdn_col_exp(x, ex, force);
@@ -824,17 +837,15 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
             for (int c = 0; c < 4; ++c) d[i][c] = xu[c & 1] * fmaf(dl[c] + dm[c], 1.f / kGdnLo, dh[c]);
         }
-        uint32_t dh[4][2], dl[4][2];
-        gdn_col_exp(d, ed, force);
-        gdn_operand(d, ed, dh, dl);
-        gdn_hand(hand.d, dh, dl, lane);
-        hand.d_up[lane] = make_float2(gdn_exp2i(ed[0]), gdn_exp2i(ed[1]));
-        named_bar_arrive(5 + pair, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hand.d[i][lane] = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
+        named_bar_arrive(kBarHand + pair, 64);
         // S <- e^G S + K^T (c d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) d[i][c] *= z.d.c[16 * i + g + (c >> 1) * 8];
+        uint32_t dh[4][2], dl[4][2];
         gdn_col_exp(d, ec, force);
         gdn_operand(d, ec, dh, dl);
         const float cu[2] = {gdn_exp2i(ec[0]), gdn_exp2i(ec[1])};
@@ -848,11 +859,11 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t fk[4];
-                    ldmatrix_x4_t(fk, z.k[0] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
+                    ldmatrix_x4_t(fk, z.kq.k[0] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
                     mma_f16(nh[e], fk, dh[j][0], dh[j][1]);
                     mma_f16(nl[e], fk, dl[j][0], dl[j][1]);
                     if constexpr (kSplit) {
-                        ldmatrix_x4_t(fk, z.k[kSplit] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
+                        ldmatrix_x4_t(fk, z.kq.k[kSplit] + (j * 16 + krow) * kLd + (i + e) * 16 + kcol);
                         mma_f16(nl[e], fk, dh[j][0], dh[j][1]);
                     }
                 }
@@ -873,8 +884,9 @@ __global__ void __launch_bounds__(384, 1) gdn_chunk_scan_kernel(const GdnScanArg
 // Tokens per segment: what the prep kernel writes for a segment is still in L2 when the scan reads it.
 constexpr int64_t kGdnSegBytes = int64_t(96) << 20;
 static int64_t gdn_chunk_bytes(bool f32, int k_heads, int v_heads, int head_dim) {
-    return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * (int64_t)(4 * 64 * head_dim * 2)
-               : v_heads * (int64_t)sizeof(GdnChunkData<false>);
+    const int64_t row = 2 * 64 * (head_dim + 8) * (int64_t)sizeof(__half);  // of a GdnKq, K and Q
+    return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * 2 * row
+               : v_heads * (int64_t)sizeof(GdnChunkData<false>) + k_heads * row;
 }
 static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
     const int64_t n = kGdnSegBytes / gdn_chunk_bytes(f32, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
@@ -898,7 +910,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
     GdnScanArgs sa;
     pa.x = sa.x = a;
     pa.data = ws;
-    pa.kq = reinterpret_cast<__half*>(ws + seg * a.v_heads * (int64_t)sizeof(GdnChunkData<kSplit>));
+    pa.kq = ws + seg * a.v_heads * (int64_t)sizeof(GdnChunkData<kSplit>);
     sa.data = pa.data;
     sa.kq = pa.kq;
     sa.state_in = a.state_in;
@@ -908,7 +920,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
         sa.t1 = t1;
         const int64_t chunks = (t1 - t0 + kGdnChunk - 1) / kGdnChunk;
         launch_k(prep, (unsigned)(chunks * a.k_heads), 128, prep_smem, stream, pa);
-        launch_k(scan, a.v_heads * (HD / 32), 384, scan_smem, stream, sa);
+        launch_k(scan, a.v_heads * (HD / 32), 288, scan_smem, stream, sa);
         sa.state_in = a.state_out;
     }
     return launch_status();

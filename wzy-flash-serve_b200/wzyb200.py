@@ -474,18 +474,22 @@ def k_rope_kv_append(k, k_gamma, v, cos_tab, sin_tab, T, kv_heads, head_dim, cac
         call("wzyb_k_rope_kv_append_f16" if f16 else "wzyb_k_rope_kv_append_f32", *args)
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
 def _raw_stream(stream, index):
     """The cudaStream_t of `stream`, or of the current stream of device `index`."""
-    if stream is not None:
-        return stream.cuda_stream
+    return _current_raw_stream(index) if stream is None else stream.cuda_stream
+
+
+def _torch_names():
+    """torch's float16, float32, int32 and current-stream query, looked up once (a decoded token's calls are
+    short enough for repeated imports and attribute chains to show)."""
+    global _f16, _f32, _i32, _current_raw_stream
     import torch
 
-    return torch._C._cuda_getCurrentRawStream(index)
+    _f16, _f32, _i32 = torch.float16, torch.float32, torch.int32
+    _current_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+_f16 = _f32 = _i32 = _current_raw_stream = None
 
 
 def kv_attn_workspace_bytes(T, q_heads, kv_heads, head_dim) -> int:
@@ -493,36 +497,33 @@ def kv_attn_workspace_bytes(T, q_heads, kv_heads, head_dim) -> int:
     return int(lib().wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim))
 
 
-def _elem_size(q):
-    """2 for float16, 4 for float32 tensors on a CUDA device."""
-    size = {"torch.float16": 2, "torch.float32": 4}.get(str(q.dtype))
-    _need(size is not None and q.is_cuda, "expected float16 or float32 tensors on a CUDA device")
-    return size
-
-
 def _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace):
-    import torch
-
-    T, q_heads, head_dim = shape = q.shape
+    if _f16 is None:
+        _torch_names()
+    dt, shape = q.dtype, q.shape
+    if not (q.is_cuda and (dt is _f16 or dt is _f32) and len(shape) == 3):
+        raise ValueError("q: expected a float16 or float32 [T, q_heads, head_dim] tensor on a CUDA device")
+    T, q_heads, head_dim = shape
     qr, qh, qe = q.stride()
     orow, oh, oe = out.stride()
-    _need(out.shape == shape and out.dtype == q.dtype and out.device == q.device, "out: expected q's shape, type and device")
-    _need(qe == 1 and oe == 1, "q and out: the head dimension must be contiguous")
-    _need(d_base_pos is None or (d_base_pos.dtype == torch.int32 and d_base_pos.is_cuda), "d_base_pos: expected int32 on the device")
+    if not (out.dtype is dt and out.shape == shape and out.is_cuda and qe == 1 and oe == 1):
+        raise ValueError("out: expected q's shape, type and device, and both contiguous in the head dimension")
+    lse_at = pos_at = ws_at = ws_bytes = 0
     if lse is not None:
-        _need(lse.shape == shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous() and lse.is_cuda,
-              "lse: expected a contiguous float32 [T, q_heads] tensor")
-    return _KV_ATTN_PACK(q.data_ptr(), q_heads, qh, qr, out.data_ptr(), oh, orow, 0 if lse is None else lse.data_ptr(),
-                         ctypes.addressof(cache), source, kv_heads, head_dim,
-                         0 if d_base_pos is None else d_base_pos.data_ptr(), pos_offset, window, sinks,
-                         head_dim**-0.5 if scale is None else scale, *_workspace(workspace))
-
-
-def _workspace(ws):
-    if ws is None:
-        return 0, 0
-    _need(ws.is_contiguous() and ws.is_cuda, "workspace must be contiguous and on the device")
-    return ws.data_ptr(), ws.numel() * ws.element_size()
+        if not (lse.dtype is _f32 and lse.shape == (T, q_heads) and lse.is_cuda and lse.is_contiguous()):
+            raise ValueError("lse: expected a contiguous float32 [T, q_heads] tensor on the device")
+        lse_at = lse.data_ptr()
+    if d_base_pos is not None:
+        if not (d_base_pos.dtype is _i32 and d_base_pos.is_cuda):
+            raise ValueError("d_base_pos: expected int32 on the device")
+        pos_at = d_base_pos.data_ptr()
+    if workspace is not None:
+        if not (workspace.is_cuda and workspace.is_contiguous()):
+            raise ValueError("workspace: expected a contiguous tensor on the device")
+        ws_at, ws_bytes = workspace.data_ptr(), workspace.nbytes
+    return _KV_ATTN_PACK(q.data_ptr(), q_heads, qh, qr, out.data_ptr(), oh, orow, lse_at, ctypes.addressof(cache), source,
+                         kv_heads, head_dim, pos_at, pos_offset, window, sinks,
+                         head_dim**-0.5 if scale is None else scale, ws_at, ws_bytes), T
 
 
 def kv_attn(q, out, cache: KvCache, kv_heads, window, sinks=0, scale=None, source=KV_RING, d_base_pos=None,
@@ -530,12 +531,11 @@ def kv_attn(q, out, cache: KvCache, kv_heads, window, sinks=0, scale=None, sourc
     """Attention of the T tokens of q [T, q_heads, head_dim] (fp16 or fp32, any head and token stride) over the
     INT8 cache they were appended to: each sees the last `window` positions up to its own and the first
     `sinks`. scale defaults to head_dim**-0.5; workspace: kv_attn_workspace_bytes(...) bytes on the device."""
-    f16 = _elem_size(q) == 2
-    args = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
-    fn = "wzyb_kv_attn_f16" if f16 else "wzyb_kv_attn_f32"
-    rc = getattr(lib(), fn)(args, q.shape[0], _raw_stream(stream, q.device.index))
+    args, T = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    L = lib()
+    rc = (L.wzyb_kv_attn_f16 if q.dtype is _f16 else L.wzyb_kv_attn_f32)(args, T, _raw_stream(stream, q.get_device()))
     if rc:
-        check(fn, rc)
+        check("wzyb_kv_attn", rc)
 
 
 def kv_tree_attn(q, out, cache: KvCache, drafts: KvCache, mask, kv_heads, window, depth, sinks=0, scale=None,
@@ -543,20 +543,16 @@ def kv_tree_attn(q, out, cache: KvCache, drafts: KvCache, mask, kv_heads, window
     """Attention of drafted nodes q [N, q_heads, head_dim]: node i stands at base + depth[i] over the `base`
     committed tokens of the cache and sees the drafts whose bit is set in mask [N, ceil(N / 32)] (int32 words);
     the drafts' k, v are cells 0..N-1 of the `drafts` ring."""
-    import torch
-
-    f16 = _elem_size(q) == 2
-    args = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
-    n = q.shape[0]
-    _need(mask.shape == (n, (n + 31) // 32) and mask.dtype == torch.int32 and mask.is_contiguous() and mask.is_cuda,
-          "mask: expected a contiguous int32 [N, ceil(N / 32)] tensor")
-    _need(depth.shape == (n,) and depth.dtype == torch.int32 and depth.is_contiguous() and depth.is_cuda,
-          "depth: expected a contiguous int32 [N] tensor")
-    fn = "wzyb_kv_tree_attn_f16" if f16 else "wzyb_kv_tree_attn_f32"
-    rc = getattr(lib(), fn)(args, ctypes.addressof(drafts), mask.data_ptr(), depth.data_ptr(), n,
-                            _raw_stream(stream, q.device.index))
+    args, n = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    if not (mask.dtype is _i32 and mask.shape == (n, (n + 31) // 32) and mask.is_cuda and mask.is_contiguous()):
+        raise ValueError("mask: expected a contiguous int32 [N, ceil(N / 32)] tensor on the device")
+    if not (depth.dtype is _i32 and depth.shape == (n,) and depth.is_cuda and depth.is_contiguous()):
+        raise ValueError("depth: expected a contiguous int32 [N] tensor on the device")
+    L = lib()
+    rc = (L.wzyb_kv_tree_attn_f16 if q.dtype is _f16 else L.wzyb_kv_tree_attn_f32)(
+        args, ctypes.addressof(drafts), mask.data_ptr(), depth.data_ptr(), n, _raw_stream(stream, q.get_device()))
     if rc:
-        check(fn, rc)
+        check("wzyb_kv_tree_attn", rc)
 
 
 def gdn_delta_rule_workspace_bytes(T, k_heads, v_heads, head_dim=128) -> int:
@@ -569,30 +565,41 @@ def gdn_delta_rule(q, k, v, g, beta, o, state_out, state_in=None, state_snaps=No
     """The gated delta rule over q, k [T, k_heads, d], v, o [T, v_heads, d] (fp16 or fp32; token strides free),
     g, beta [T, v_heads] fp32, states [v_heads, d (v), d (k)] fp32 (state_in None: zeros; may be state_out).
     state_snaps [T, v_heads, d, d]: the state after every token. scale defaults to d**-0.5."""
-    import torch
-
-    f16 = _elem_size(q) == 2
-    T, k_heads, d = q.shape
-    v_heads = v.shape[1]
-    dt, f32, st = q.dtype, torch.float32, (v_heads, d, d)
-    strides = []
-    for t, h in ((q, k_heads), (k, k_heads), (v, v_heads), (o, v_heads)):
-        row, head, elem = t.stride()
-        _need(t.dtype == dt and t.shape == (T, h, d) and t.is_cuda, "q, k [T, k_heads, d], v, o [T, v_heads, d]: shapes or types differ")
-        _need(elem == 1 and (head == d or h == 1), "q, k, v, o: the heads of a token must be contiguous")
-        strides.append(row)
-    for t, shape in ((g, (T, v_heads)), (beta, (T, v_heads)), (state_out, st), (state_in, st), (state_snaps, (T, *st))):
-        _need(t is None or (t.dtype == f32 and t.shape == shape and t.is_contiguous() and t.is_cuda),
-              "g, beta and the states: expected contiguous float32 tensors of their shapes")
-    args = _GDN_DELTA_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides[:3], g.data_ptr(), beta.data_ptr(),
-                           0 if state_in is None else state_in.data_ptr(), state_out.data_ptr(),
-                           0 if state_snaps is None else state_snaps.data_ptr(), o.data_ptr(), strides[3], k_heads,
-                           v_heads, d, d**-0.5 if scale is None else scale, 1 if qk_l2norm else 0, l2_eps,
-                           *_workspace(workspace))
-    fn = "wzyb_gdn_delta_rule_f16" if f16 else "wzyb_gdn_delta_rule_f32"
-    rc = getattr(lib(), fn)(args, T, _raw_stream(stream, q.device.index))
+    if _f16 is None:
+        _torch_names()
+    dt, qk, vo = q.dtype, q.shape, v.shape
+    if not (q.is_cuda and (dt is _f16 or dt is _f32) and len(qk) == 3 and k.dtype is dt and k.shape == qk and k.is_cuda):
+        raise ValueError("q, k: expected float16 or float32 [T, k_heads, d] tensors on a CUDA device")
+    T, k_heads, d = qk
+    if not (v.dtype is dt and len(vo) == 3 and vo[0] == T and vo[2] == d and v.is_cuda and o.dtype is dt and o.shape == vo
+            and o.is_cuda):
+        raise ValueError("v, o: expected [T, v_heads, d] tensors of q's type on the device")
+    v_heads = vo[1]
+    (qr, qh, qe), (kr, kh, ke), (vr, vh, ve), (orow, oh, oe) = q.stride(), k.stride(), v.stride(), o.stride()
+    if not (qe == ke == ve == oe == 1 and (k_heads == 1 or qh == kh == d) and (v_heads == 1 or vh == oh == d)):
+        raise ValueError("q, k, v, o: the heads of a token must be contiguous")
+    th, st = (T, v_heads), (v_heads, d, d)
+    if not (g.dtype is _f32 and beta.dtype is _f32 and g.shape == th and beta.shape == th and g.is_cuda and beta.is_cuda
+            and g.is_contiguous() and beta.is_contiguous()):
+        raise ValueError("g, beta: expected contiguous float32 [T, v_heads] tensors on the device")
+    at = [0, 0, 0]
+    for i, (t, shape) in enumerate(((state_in, st), (state_out, st), (state_snaps, (T, v_heads, d, d)))):
+        if t is not None:
+            if not (t.dtype is _f32 and t.shape == shape and t.is_cuda and t.is_contiguous()):
+                raise ValueError("states: expected contiguous float32 [v_heads, d, d] (snapshots [T, v_heads, d, d]) on the device")
+            at[i] = t.data_ptr()
+    ws_at = ws_bytes = 0
+    if workspace is not None:
+        if not (workspace.is_cuda and workspace.is_contiguous()):
+            raise ValueError("workspace: expected a contiguous tensor on the device")
+        ws_at, ws_bytes = workspace.data_ptr(), workspace.nbytes
+    args = _GDN_DELTA_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), qr, kr, vr, g.data_ptr(), beta.data_ptr(), *at,
+                           o.data_ptr(), orow, k_heads, v_heads, d, d**-0.5 if scale is None else scale,
+                           1 if qk_l2norm else 0, l2_eps, ws_at, ws_bytes)
+    L = lib()
+    rc = (L.wzyb_gdn_delta_rule_f16 if dt is _f16 else L.wzyb_gdn_delta_rule_f32)(args, T, _raw_stream(stream, q.get_device()))
     if rc:
-        check(fn, rc)
+        check("wzyb_gdn_delta_rule", rc)
 
 
 def rope_table(cos_tab, sin_tab, rows, rot_dims=64, theta=1e7, stream=None):
