@@ -44,6 +44,7 @@ struct KvAttnArgs {
     int64_t window, sinks;
     float scale_log2;  // scale * log2(e)
     uint64_t ring_div, ring_recip;
+    int ring_step;  // ring_div, or the largest int where cells do not wrap
     int splits;
     float* part_o;   // [splits, T * q_heads, HD]
     float2* part_ml;  // [splits, T * q_heads]: running maximum (log2 units) and sum
@@ -342,16 +343,33 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
     // K of the next tile is on its way while the current one is worked through (its registers are free once the
     // scores are there); V of the current one while its scores are computed.
     KeyTile kt = {};
-    int my_cell = 0;
+    int my_cell = 0, range_end = 0, range_hi = 0, cell_limit = 0;  // the current range's end in tiles and positions
+    Planes pl = {};
     uint4 kr[2][NG];
     uint16_t ksb[2][NG];
     auto load_k = [&](int it) {
-        kt = key_tile<kN>(plan, it);
-        // lanes 0..15 find the tile's cells; a key past the tile's end takes the first one's cell (its scales
-        // count as 0 and its scores as -inf)
+        // Inside a range the next tile's cells are kWarps * kN further on (one step back where the ring wraps: a tile
+        // holds no more keys than the ring). Lanes 0..15 have a key each; one past the tile's end has the first
+        // one's cell (its scales count as 0 and its scores as -inf).
         const int mine = lane & 15;
-        my_cell = (int)cell_of(a, kt.draft, kt.pos + (mine < kt.count ? mine : 0));
-        const Planes pl = planes_of<HD>(a, kt.draft, head);
+        if (it < range_end && kt.count == kN && a.ring_step >= kWarps * kN) {
+            kt.pos += kWarps * kN;
+            kt.count = min(kN, range_hi - kt.pos);
+            my_cell += kWarps * kN;
+            if (my_cell >= cell_limit) my_cell -= a.ring_step;
+            if (kt.count < kN) my_cell = __shfl_sync(0xffffffffu, my_cell, mine < kt.count ? mine : 0);
+        } else {
+            int r = 0;
+#pragma unroll
+            for (int n = 1; n < kAttnMaxRanges; ++n)
+                if (n < plan.ranges && it >= plan.first[n]) r = n;
+            kt = key_tile<kN>(plan, it);
+            range_end = plan.first[r + 1];
+            range_hi = plan.hi[r];
+            pl = planes_of<HD>(a, kt.draft, head);
+            cell_limit = kt.draft || a.from_full ? 0x7FFFFFFF : (int)a.c.ring_cap;
+            my_cell = (int)cell_of(a, kt.draft, kt.pos + (mine < kt.count ? mine : 0));
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int cell = __shfl_sync(0xffffffffu, my_cell, g + 8 * i);
@@ -360,6 +378,8 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
                 kr[i][n] = __ldg(reinterpret_cast<const uint4*>(pl.kq + (int64_t)cell * kvd + n * 64 + t4 * 16));
             load_scale_bits<NG>(pl.ks + (int64_t)cell * spc, ksb[i]);
         }
+        // the tile's V rows, which are loaded a turn later, to L2 (a 128-byte line per lane)
+        if (HD > 128 || lane < 16) prefetch_l2(pl.vq + (int64_t)my_cell * kvd + (lane >> 4) * 128);
     };
     if (tb + warp < te) load_k(tb + warp);
     for (int it = tb + warp; it < te; it += kWarps) {
@@ -368,7 +388,6 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
         uint16_t vsb[2][NG];
         float ks[2][NG], vs[2][NG];
         {
-            const Planes pl = planes_of<HD>(a, now.draft, head);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int cell = __shfl_sync(0xffffffffu, my_cell, 2 * t4 + (i & 1) + (i >> 1) * 8);
@@ -420,11 +439,19 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
             for (int n = 0; n < NG; ++n) vs[i][n] = __half2float(__ushort_as_half(vsb[i][n]));
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[c] *= rs[c & 1];
-        int ek[2] = {-1000, -1000}, e[2];
+        int ek[2], e[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            uint32_t top_bits = 0;  // finite fp16 scales order like their bits
 #pragma unroll
-            for (int n = 0; n < NG; ++n) ek[i] = max(ek[i], scale_exp(vs[i][n]));
+            for (int n = 0; n < NG; ++n) top_bits = max(top_bits, (uint32_t)vsb[i][n]);
+            ek[i] = scale_exp(__half2float(__ushort_as_half((uint16_t)top_bits)));
+            if (top_bits >= 0x7C00u) {  // an infinity or NaN among them
+                ek[i] = -1000;
+#pragma unroll
+                for (int n = 0; n < NG; ++n) ek[i] = max(ek[i], scale_exp(vs[i][n]));
+            }
+        }
         if (tile_unmasked<kN>(plan, now)) {  // warp-uniform
             e[0] = e[1] = max(ek[0], ek[1]);
         } else {
@@ -1506,6 +1533,7 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     a.scale_log2 = x.scale * kLog2e;
     a.ring_div = full ? 1 : (uint64_t)(c.ring_cap <= 2 * kKvSinkPin ? c.ring_cap : c.ring_cap - kKvSinkPin);
     a.ring_recip = ~0ull / a.ring_div;
+    a.ring_step = full ? 0x7FFFFFFF : (int)a.ring_div;
     // the most keys that a row tile can see, known here; a split takes at least two key tiles of each warp
     int64_t keys = (x.sinks < kMaxPos ? x.sinks : kMaxPos) + (a.window < kMaxPos ? a.window : kMaxPos) + T_;
     const int64_t held = full || c.ring_cap > c.max_ctx ? c.max_ctx : c.ring_cap;
