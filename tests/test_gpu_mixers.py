@@ -472,3 +472,21 @@ def test_gdn_in_two_calls_and_no_tokens(wz, dtype):
     big = float(s.abs().max() + v.abs().max())
     assert (s - s2).abs().max() <= big * (T + 64) * 2.0**-21
     assert (o.float() - o2.float()).abs().max() <= big * (2.0**-9 if dtype == torch.float16 else 2.0**-12)
+
+
+# ---- both mixers together ------------------------------------------------------------------------
+
+
+def test_example_chunks_and_tokens_agree_with_one_chunk(wz):
+    """The example's prompt in chunks and its tokens one by one give what one long chunk gives: attention to the
+    rounding of k's appended codes and the fp16 outputs, the delta rule to its own bounds."""
+    import example_mixers as ex
+
+    # attention outputs are means of values of size 1 with weights off by 2^-11 and rounded to fp16: 2^-9 of the largest
+    kw = dict(ring=9000, max_ctx=16384, window=300, sinks=8)
+    ya, yb, tree, attn, gdn = ex.run(prompt=640, chunk=160, decoded=5, **kw)
+    za, zb, *_ = ex.run(prompt=645, chunk=645, decoded=0, **kw)
+    assert (ya.float() - za.float()).abs().max() <= 2.0**-9 * za.float().abs().max()
+    assert (yb.float() - zb.float()).abs().max() <= 2.0**-8 * zb.float().abs().max()
+    assert int(attn.pos) == 647 and torch.isfinite(tree).all()
+    assert wz.read_faults() == 0
