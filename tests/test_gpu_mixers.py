@@ -490,3 +490,23 @@ def test_example_chunks_and_tokens_agree_with_one_chunk(wz):
     assert (yb.float() - zb.float()).abs().max() <= 2.0**-8 * zb.float().abs().max()
     assert int(attn.pos) == 647 and torch.isfinite(tree).all()
     assert wz.read_faults() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attn_long_context_sums_do_not_drift(wz, dtype):
+    """Values that all add up: a chunk that one CTA walks 100,000 keys for (no split) stays within the usual bound."""
+    n, T, qh, kvh, hd = 100_000, 1200, 32, 2, 64
+    r = gen(20)
+    x = torch.randn(n, kvh, 64, generator=r, device=DEV)
+    planes = []
+    for y in (x, 3 + torch.randn(n, kvh, 64, generator=r, device=DEV)):
+        s = (y.abs().amax(-1) / 127).half()
+        planes += [torch.round(y / s.float().unsqueeze(-1)).clamp(-127, 127).to(torch.int8).reshape(n, kvh * hd), s.view(torch.int16)]
+    tiny = [torch.zeros(16, p.shape[1], dtype=p.dtype, device=DEV) for p in planes]
+    q = torch.randn(T, qh, hd, generator=r, device=DEV).to(dtype)
+    out, lse = torch.empty_like(q), torch.zeros(T, qh, device=DEV)
+    assert wz.kv_attn_workspace_bytes(T, qh, kvh, hd) == 0  # not split
+    wz.kv_attn(q, out, wz.kv_cache(*tiny, 16, n, *planes), kvh, n, source=wz.KV_FULL, pos_offset=n - T, lse=lse)
+    at = [0, 7, T - 1]
+    want = ref.attention(q[at], planes, kvh, hd, hd**-0.5, [list(range(n - T + t + 1)) for t in at])
+    check_attention(q[at], out[at], lse[at], want)

@@ -626,16 +626,17 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 // 0..255 hold a tile's scores, 64 per 64-element group (the groups' scales differ per key, so each group's
 // products have their own accumulator), and then, in the same columns, the weights: per group the fp16 copy of
 // p * vs (and for fp32 calls its second part); columns 256..511 hold the tile's p V.
-//   softmax warps (8 for fp32 calls, 16 for fp16): a row is 2 or 4 lanes, each with a share of the tile's keys:
+//   softmax warps (8 or 16): a row is 2 or 4 lanes, each with a share of the tile's keys:
 //               scores from tensor memory, running maximum, exponentials, weights back to tensor memory
 //   cell warps (4): the tile's codes from global memory (K a tile ahead, V a product ahead, in registers), widened to fp16 into
 //               128-byte rows of shared memory with the 128-byte swizzle. Keys and values have the same layout:
 //               K is read with the dimension contracted (K-major), V with the keys contracted (MN-major)
 //   one warp    issues the MMAs: S_g = Q_g K_g^T, then o_g = P_g V_g with P_g from tensor memory
-// fp16 calls sum o in tensor memory and scale it there when a row's maximum moves. The tensor cores cut their
-// sums off towards zero, which is a drift of about 2^-25 per 16 keys: fine for an fp16 result, not for an fp32
-// one. fp32 calls take every tile's p V from tensor memory onto fp32 registers instead (64 to 128 a lane,
-// which is why they have 8 softmax warps).
+// o is summed in tensor memory (and scaled there when a row's maximum moves), or with kReg every tile's p V is
+// taken from there onto fp32 registers (up to 128 a lane, so with 8 softmax warps). The tensor cores cut their sums off
+// towards zero, up to 2^-23 per 16 keys (measured: 1.7e-3 of a value-biased o over 262,144 keys, 2e-4 over 32,768;
+// in registers 2e-4, the output's rounding, at any length). So fp32 calls, and fp16 calls in which a CTA may walk more
+// than kAttnDriftKeys, sum in registers; shorter fp16 calls in tensor memory, which is faster.
 // Every wait is bounded.
 // ----------------------------------------------------------------------------------------------------
 // Issued by one elected lane of a converged warp: the warp-uniform operands stay in uniform registers (inside an
@@ -744,11 +745,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
 
 constexpr int kTileMasked = 1, kTileDraft = 2, kTileBad = 4;  // bad: a value scale is infinite or NaN
 
-template <typename T, int HD>
+template <typename T, int HD, bool kReg>
 struct TcSmem {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kRows = 128, kN = 64, NG = HD / 64;
-    static constexpr int kSW = kSplit ? 8 : 16, kParts = kSW / 4;  // softmax warps; lanes per row
+    static constexpr int kSW = kReg ? 8 : 16, kParts = kSW / 4;  // softmax warps; lanes per row
     static constexpr int kThreads = (kSW + 8) * 32;
     static constexpr int kPairs = (NG + 1) / 2;  // groups are handed on two at a time
     // [group][row][64 dims], 128-byte rows, swizzled
@@ -777,16 +778,17 @@ __device__ __forceinline__ int64_t q_offset(const KvAttnArgs& a, int head, int r
     return t * a.q_row + (int64_t)(head * a.G + (row - t * a.G)) * a.q_head;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
+template <typename T, int HD, bool kReg>
+__global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile_kernel(const KvAttnArgs a) {
     pdl_begin();
-    using S = TcSmem<T, HD>;
+    using S = TcSmem<T, HD, kReg>;
     constexpr bool kSplit = S::kSplit;
+    static_assert(kReg || !kSplit, "fp32 sums stay in registers");
     constexpr int NG = S::NG, kN = S::kN, kSW = S::kSW, kParts = S::kParts, kPairs = S::kPairs, kKeys = kN / kParts, kDims = HD / kParts;
     extern __shared__ __align__(1024) uint8_t attn_smem[];
     S& sm = *reinterpret_cast<S*>(attn_smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int split = blockIdx.x, row0 = (gridDim.y - 1 - blockIdx.y) * S::kRows, head = blockIdx.z;
+    const int split = blockIdx.y, row0 = (gridDim.x - 1 - blockIdx.x) * S::kRows, head = blockIdx.z;
     const int rows = a.T * a.G;
     const int64_t base = (a.d_base_pos ? (int64_t)__ldg(a.d_base_pos) : 0) + a.pos_offset;
 
@@ -869,10 +871,10 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
     // all 512 columns were asked for, so they start at 0; the constant keeps the MMAs' operands immediate
     constexpr uint32_t tmem = 0;
 
-    // registers: launched with 128 (fp32, 512 threads) or 80 (fp16, 768 threads) each; 256 x 208 + 128 x 64 + 128 x 32
+    // registers: launched with 128 (512 threads) or 80 (768 threads) each; 256 x 208 + 128 x 64 + 128 x 32
     // and 512 x 96 + 128 x 64 + 128 x 32 are the same totals
     if (warp < kSW) {
-        if constexpr (kSplit)
+        if constexpr (kReg)
             asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         else
             asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
@@ -882,8 +884,8 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
         const int t = min(row, rows - 1) / a.G;
         const RowSpan span = row_span(a, base, t);
         const float up = kSplit ? sm.row_up[r] : 1.f;
-        float o[kSplit ? kDims : 1];
-        if constexpr (kSplit) {
+        float o[kReg ? kDims : 1];
+        if constexpr (kReg) {
 #pragma unroll
             for (int i = 0; i < kDims; ++i) o[i] = 0.f;
         }
@@ -891,7 +893,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
         int E = -1000;
         auto unit = [](int e) { return e <= -1000 ? 7 : e; };  // while only scales of 0 have been seen
         bool ok = true;
-        // fp32 calls: the previous tile's p V onto o
+        // sums in registers: the previous tile's p V onto o
         auto drain = [&](uint32_t parity) {
             ok = tc_wait_warp(&sm.o_full, parity);
             if (!ok) return;
@@ -912,7 +914,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
         };
         for (int it = tb; it < te; ++it) {
             const int n = it - tb, b = n & 1;
-            if constexpr (kSplit) {
+            if constexpr (kReg) {
                 if (n > 0) {
                     drain(b ^ 1);
                     if (!ok) break;
@@ -993,7 +995,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
                 m = top;
                 E = e;
             }
-            if constexpr (!kSplit) {
+            if constexpr (!kReg) {
                 if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                     ok = tc_wait_warp(&sm.o_full, b ^ 1);
                     if (!ok) break;
@@ -1064,7 +1066,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
             }
         }
         if (te > tb && ok) {
-            if constexpr (kSplit) {
+            if constexpr (kReg) {
                 drain((te - tb - 1) & 1);
             } else {
                 ok = tc_wait_warp(&sm.o_full, (te - tb - 1) & 1);
@@ -1101,7 +1103,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
 #pragma unroll
                 for (int i = 0; i < kCols; i += 16) {
                     float x[16];
-                    if constexpr (kSplit) {
+                    if constexpr (kReg) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) x[j] = o[c + i + j] * norm;
                     } else {
@@ -1275,7 +1277,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD>::kThreads, 1) kv_attn_tile_kerne
                             tc_mma_ts(d, p + 32 + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, x > 0);
                         tc_mma_ts_down11(d, p, vd + g * kKG, kTcIdescBMn);
                     } else {
-                        tc_mma_ts(d, p, vd + g * kKG, kTcIdescBMn, n > 0);
+                        tc_mma_ts(d, p, vd + g * kKG, kTcIdescBMn, !kReg && n > 0);
                     }
 #pragma unroll
                     for (int x = 1; x < 4; ++x) tc_mma_ts(d, p + x * 8, vd + g * kKG + x * (2048 >> 4), kTcIdescBMn, 1);
@@ -1441,18 +1443,29 @@ static AttnShape attn_shape(int64_t T, int q_heads, int kv_heads) {
     return s;
 }
 
+// Keys that one CTA may add up in tensor memory: a drift of 2^-23 * 16384 / 16, half an fp16 rounding.
+constexpr int64_t kAttnDriftKeys = 16384;
+template <typename T, int HD, bool kReg>
+static int launch_tiles(const KvAttnArgs& a, dim3 grid, cudaStream_t stream) {
+    using S = TcSmem<T, HD, kReg>;
+    const auto kern = kv_attn_tile_kernel<T, HD, kReg>;
+    const int rc = ensure_smem((const void*)kern, (int)sizeof(S));
+    if (rc == WZYB_OK) launch_k(kern, grid, S::kThreads, sizeof(S), stream, a);
+    return rc;
+}
 template <typename T, int HD>
-static int launch_attn(KvAttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-    const dim3 grid(a.splits, s.row_tiles, a.kv_heads);
+static int launch_attn(KvAttnArgs& a, const AttnShape& s, int64_t keys, cudaStream_t stream) {
     int rc = WZYB_OK;
     if (s.few) {
-        launch_k(kv_attn_few_kernel<T, HD>, grid, 128, 0, stream, a);
+        launch_k(kv_attn_few_kernel<T, HD>, dim3(a.splits, s.row_tiles, a.kv_heads), 128, 0, stream, a);
     } else {
-        const auto kern = kv_attn_tile_kernel<T, HD>;
-        const int smem = (int)sizeof(TcSmem<T, HD>);
-        rc = ensure_smem((const void*)kern, smem);
+        const dim3 grid(s.row_tiles, a.splits, a.kv_heads);
+        if (sizeof(T) == 2 && keys / a.splits <= kAttnDriftKeys) {
+            if constexpr (sizeof(T) == 2) rc = launch_tiles<T, HD, false>(a, grid, stream);
+        } else {
+            rc = launch_tiles<T, HD, true>(a, grid, stream);
+        }
         if (rc != WZYB_OK) return rc;
-        launch_k(kern, grid, TcSmem<T, HD>::kThreads, smem, stream, a);
     }
     const int out_rows = a.T * a.G * a.kv_heads;
     if (a.splits > kJoinFew)
@@ -1546,9 +1559,9 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
         a.part_o = reinterpret_cast<float*>(a.part_ml + (((int64_t)a.splits * rows + 1) & ~int64_t(1)));
     }
     switch (x.head_dim) {
-        case 64: return launch_attn<T, 64>(a, s, stream);
-        case 128: return launch_attn<T, 128>(a, s, stream);
-        default: return launch_attn<T, 256>(a, s, stream);
+        case 64: return launch_attn<T, 64>(a, s, keys, stream);
+        case 128: return launch_attn<T, 128>(a, s, keys, stream);
+        default: return launch_attn<T, 256>(a, s, keys, stream);
     }
 }
 
