@@ -893,8 +893,10 @@ static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int
     const int64_t segs = n < 1 ? all : (all + n - 1) / n;
     return segs < 1 ? 1 : (all + segs - 1) / segs;  // segments of one size: a short last one costs as much as a long one's start
 }
-// Calls of at least this many tokens take the chunked form.
-constexpr int64_t kGdnChunkedFrom = 64;
+// Calls of at least this many tokens take the chunked form. Chunked / token by token, us per call: fp16 16/32 heads of
+// 128, 64 tokens 22 / 21, 96 26 / 30, 256 34 / 78; fp32 16/48 heads 64 tokens 38 / 32, 96 45 / 47; fp32 2/6 heads of
+// 64, 96 tokens 28 / 23, 128 28 / 31.
+constexpr int64_t kGdnChunkedFrom = 96;
 
 template <typename T, int HD>
 static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t stream) {

@@ -1425,17 +1425,25 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
     }
 }
 
-// Which kernel a call takes and how far the keys may be split, from the sizes alone (the key count is only
-// known on the device). The workspace function and the launcher share it.
+// Which kernel a call takes and how far its keys may be split, from the sizes alone (how many keys there are is only
+// known on the device; `keys` is the most there can be). us per call, few-row kernel / tile kernel:
+//   rows per kv head    24          32          48         64          96
+//   2x256 fp16   2K     10 / 15     10 / 15     12 / 16    12 / 16     15 / 23 (fp32)
+//               28K     24 / 29     28 / 29     39 / 29    48 / 30     84 / 43 (fp32)
+//              131K     83 / 106   105 / 106   152 / 108  198 / 108   359 / 152 (fp32)
+//   2x128 fp16 131K     62 / 65     79 / 68;   8x128 fp16 28K  46 / 59,  75 / 59
+// so few rows are up to 32 of head_dim 256 and up to 24 of the others, and up to 96 where no more than 6144 keys
+// can be seen (the lines through these figures cross at 6200 to 8800).
 constexpr int kAttnSms = 148;  // two CTAs per SM for few rows, one for many
+constexpr int64_t kAttnFewKeys = 6144, kAttnFewKeysRows = 96;
 struct AttnShape {
     bool few;
     int tile_rows, row_tiles, max_splits;
 };
-static AttnShape attn_shape(int64_t T, int q_heads, int kv_heads) {
+static AttnShape attn_shape(int64_t T, int q_heads, int kv_heads, int head_dim, int64_t keys) {
     AttnShape s;
     const int64_t rows = T * (q_heads / kv_heads);
-    s.few = rows <= 16;
+    s.few = rows <= (head_dim == 256 ? 32 : 24) || (rows <= kAttnFewKeysRows && keys <= kAttnFewKeys);
     s.tile_rows = s.few ? 8 : 128;
     s.row_tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
     const int64_t ctas = (int64_t)s.row_tiles * kv_heads, most = s.few ? 2 * kAttnSms : kAttnSms;
@@ -1512,7 +1520,11 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
         ((uintptr_t)depth & 3) != 0)
         return WZYB_ERR_ALIGN;
     if (T_ == 0) return WZYB_OK;
-    const AttnShape s = attn_shape(T_, x.q_heads, x.kv_heads);
+    // the most keys that a row tile can see, as far as the host knows
+    const int64_t window = x.window < kMaxPos ? x.window : kMaxPos, sinks = x.sinks < kMaxPos ? x.sinks : kMaxPos;
+    const int64_t held = full || c.ring_cap > c.max_ctx ? c.max_ctx : c.ring_cap, span = sinks + window + T_;
+    const int64_t keys = (span < held ? span : held) + (tree ? T_ : 0);
+    const AttnShape s = attn_shape(T_, x.q_heads, x.kv_heads, x.head_dim, keys);
     if (s.max_splits > 1) {
         if (!x.workspace) return WZYB_ERR_NULL;
         if (!aligned16(x.workspace)) return WZYB_ERR_ALIGN;
@@ -1547,11 +1559,8 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     a.ring_div = full ? 1 : (uint64_t)(c.ring_cap <= 2 * kKvSinkPin ? c.ring_cap : c.ring_cap - kKvSinkPin);
     a.ring_recip = ~0ull / a.ring_div;
     a.ring_step = full ? 0x7FFFFFFF : (int)a.ring_div;
-    // the most keys that a row tile can see, known here; a split takes at least two key tiles of each warp
-    int64_t keys = (x.sinks < kMaxPos ? x.sinks : kMaxPos) + (a.window < kMaxPos ? a.window : kMaxPos) + T_;
-    const int64_t held = full || c.ring_cap > c.max_ctx ? c.max_ctx : c.ring_cap;
-    keys = (keys < held ? keys : held) + (tree ? T_ : 0);
-    const int64_t most = keys / (s.few ? 128 : 128) + 1;
+    // a split takes two key tiles of each warp (few rows) or of the CTA at least
+    const int64_t most = keys / 128 + 1;
     a.splits = (int)(most < s.max_splits ? most : s.max_splits);
     if (a.splits > 1) {
         const int64_t rows = T_ * x.q_heads;
@@ -1571,7 +1580,11 @@ extern "C" {
 
 int64_t wzyb_kv_attn_workspace(int64_t T, int q_heads, int kv_heads, int head_dim) {
     if (T < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 || head_dim < 1) return 0;
-    const int64_t n = wzyb::attn_shape(T, q_heads, kv_heads).max_splits;
+    int64_t n = 1;  // either kernel may be taken, by what the call's window is
+    for (const int64_t keys : {int64_t(0), int64_t(1) << 30}) {
+        const int64_t m = wzyb::attn_shape(T, q_heads, kv_heads, head_dim, keys).max_splits;
+        n = m > n ? m : n;
+    }
     return n > 1 ? n * T * q_heads * (head_dim * 4 + 8) + 16 : 0;
 }
 int wzyb_kv_attn_f16(const wzyb_kv_attn_args* a, int64_t T, wzyb_stream_t stream) {
