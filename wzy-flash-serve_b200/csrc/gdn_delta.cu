@@ -627,6 +627,14 @@ struct GdnHandOver {
     float4 d[4][32];
     float2 s_up[32];
 };
+// All of a scan CTA's shared memory; the launch asks for its size, so no part of it can lie outside.
+template <typename T, int HD>
+struct GdnScanSmem {
+    GdnScanStage<T, HD> st[2];
+    GdnHandOver<HD> hand[4];  // one per pair of warps
+    uint64_t full[2];         // a chunk's copies have landed
+};
+static_assert(sizeof(GdnScanSmem<float, 128>) <= 227 * 1024, "the largest instance fits one CTA per SM");
 template <int N>
 __device__ __forceinline__ void gdn_hand(uint4 (&to)[N][32], const uint32_t (&hi)[N][2], const uint32_t (&lo)[N][2], int lane) {
 #pragma unroll
@@ -652,16 +660,17 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
     constexpr bool kSplit = Stage::kSplit;
     constexpr int kLd = Stage::kLd, kVLd = Stage::kVLd, kM = HD / 16;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    Stage* const st = reinterpret_cast<Stage*>(smem_raw);
+    GdnScanSmem<T, HD>& sm = *reinterpret_cast<GdnScanSmem<T, HD>*>(smem_raw);
+    Stage* const st = sm.st;
     const GdnDeltaArgs& a = p.x;
     const int tid = threadIdx.x, lane = tid & 31, pair = (tid >> 5) & 3, g = lane >> 2, t4 = lane & 3;
     const int role = tid >> 7;  // 0 state, 1 output, 2 fetch
-    GdnHandOver<HD>& hand = reinterpret_cast<GdnHandOver<HD>*>(smem_raw + 2 * sizeof(Stage))[pair];
+    GdnHandOver<HD>& hand = sm.hand[pair];
     const int h = blockIdx.x / (HD / 32), c0 = (blockIdx.x % (HD / 32)) * 32;
     const int hk = h / (a.v_heads / a.k_heads);
     const int chunks = (int)((p.t1 - p.t0 + kGdnChunk - 1) / kGdnChunk);
 
-    uint64_t* const full = reinterpret_cast<uint64_t*>(smem_raw + 2 * sizeof(Stage) + 4 * sizeof(GdnHandOver<HD>) + 16);
+    uint64_t* const full = sm.full;
     if (tid == 0) {
         mbar_init(&full[0], 1);
         mbar_init(&full[1], 1);
@@ -913,7 +922,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
     const int64_t seg = gdn_seg_chunks(kSplit, a.T, a.k_heads, a.v_heads, HD);
     const auto prep = gdn_chunk_prep_kernel<T, HD>;
     const auto scan = gdn_chunk_scan_kernel<T, HD>;
-    const int prep_smem = (int)sizeof(GdnPrepSmem<T, HD>), scan_smem = (int)(2 * sizeof(GdnScanStage<T, HD>) + 4 * sizeof(GdnHandOver<HD>));
+    const int prep_smem = (int)sizeof(GdnPrepSmem<T, HD>), scan_smem = (int)sizeof(GdnScanSmem<T, HD>);
     int rc = ensure_smem((const void*)prep, prep_smem);
     if (rc == WZYB_OK) rc = ensure_smem((const void*)scan, scan_smem);
     if (rc != WZYB_OK) return rc;
