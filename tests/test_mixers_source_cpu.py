@@ -29,3 +29,16 @@ def test_dynamic_shared_memory_is_one_struct(name, kernels):
             assert re.fullmatch(rf"(.+)& sm = \*reinterpret_cast<\1\*>\({buffer}\);", line), line
     for size in re.findall(r"\w+_smem = (.{40})", text):
         assert re.match(r"\(int\)sizeof\(\w+<T, HD>\)[,;]", size), size
+
+
+def test_tensor_memory_changes_hands_between_fences():
+    """Tensor memory that one warp read or wrote and another writes or reads next: every hand-over through an mbarrier has
+    tcgen05's fence before the arrival and the other one after the wait. The score columns go from the MMA to the softmax
+    warps (s_full), among these (x_full) and back as weights (p_full)."""
+    text = re.sub(r"\s+", " ", source("kv_attn.cu"))
+    loop = text[text.index("float s[kKeys];"):text.index("sm.x_max[0][part][r] = l;")]
+    assert "tc_fence_before(); warp_arrive(&sm.x_full[warp & 3], lane);" in loop
+    assert "ok = tc_wait_warp(&sm.x_full[warp & 3], b); if (!ok) break; tc_fence_after();" in loop
+    assert "tc_wait_st(); tc_fence_before(); warp_arrive(&sm.p_full[g / 2], lane);" in loop
+    for wait in re.findall(r"tc_wait_warp\(&sm\.(?:s|x|o)_full[^;]*; if \(!ok\) break; (.{16})", loop):
+        assert wait == "tc_fence_after()"

@@ -982,10 +982,13 @@ __global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile
 #pragma unroll
             for (int i = 0; i < kKeys; ++i) top = fmaxf(top, s[i]);
             sm.x_max[b][part][r] = top * up;
+            // the warps of these 32 rows; also: their scores have been read, so weights may take their columns (a
+            // warp's weights lie where another one's scores were, so the fences order the two warps' accesses)
+            tc_fence_before();
             warp_arrive(&sm.x_full[warp & 3], lane);
-            // the warps of these 32 rows; also: their scores have been read, so weights may take their columns
             ok = tc_wait_warp(&sm.x_full[warp & 3], b);
             if (!ok) break;
+            tc_fence_after();
             top = sm.x_max[b][0][r];
 #pragma unroll
             for (int i = 1; i < kParts; ++i) top = fmaxf(top, sm.x_max[b][i][r]);
