@@ -45,7 +45,7 @@ typedef struct CUstream_st* wzyb_stream_t; /* identical to cudaStream_t */
 #define WZYB_ERR_VALUE (-5)  /* an enum / mode argument has an unknown value                   */
 
 /* ---- device fault bits (wzyb_read_faults) ------------------------------------------------ */
-#define WZYB_FAULT_WAIT_TIMEOUT 0x1u /* a TMA / mbarrier wait gave up after its limit           */
+#define WZYB_FAULT_WAIT_TIMEOUT 0x1u /* a TMA / mbarrier wait gave up after its time limit      */
 #define WZYB_FAULT_POS_RANGE 0x2u    /* a RoPE position fell outside [0, table_rows)           */
 
 /* ---- modes --------------------------------------------------------------------------------- */

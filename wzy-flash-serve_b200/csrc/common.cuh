@@ -39,6 +39,12 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
     return t;
 }
 
+__device__ __forceinline__ uint32_t globaltimer_lo_ns() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -89,6 +95,29 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
             return false;
         }
     }
+}
+
+// Like mbar_wait, for roles of a CTA that wait for long beside others that work: each poll may sleep in hardware for a
+// while (the hint, 100 us at most), so the waiting warps leave the issue slots alone (without it the attention's tile of
+// 5100 cycles took 5900). The limit is kept on the low word of the clock, which wraps after 4.3 s: a flag by which the
+// first role to give up would end the other roles' waits costs the 4096-token chunk 9 %. Where every role waits for the
+// others within a tile, they all begin the wait that runs out in the same microseconds, so the limits do not add up.
+__device__ __forceinline__ bool mbar_wait_asleep(uint64_t* bar, uint32_t parity) {
+    const uint32_t t0 = globaltimer_lo_ns();
+#pragma unroll 1
+    do {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(100000)
+            : "memory");
+        if (ok) return true;
+    } while (globaltimer_lo_ns() - t0 <= (uint32_t)kWaitLimitNs);
+    raise_fault(WZYB_FAULT_WAIT_TIMEOUT);
+    return false;
 }
 
 // Like mbar_wait, but against an absolute %globaltimer deadline and without raising a fault:

@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 // softmax take turns, and that sum bounds the kernel. Measured with 16/2 heads of 256: 4096 fp16 tokens with a window
 // of 8192 in 1419 us, a tile 4200 cycles (scores 1000, softmax and weights 2700, p V 500); 64 fp32 nodes of 24/2 heads
 // over 131,072 cells in 755 us, a tile 6000 cycles (scores 2000, softmax with split weights 3600), kReg.
-// Every wait is bounded.
+// Every wait is bounded. A role whose wait gives up ends its loop; the others, which wait for it, run out beside it.
 // ----------------------------------------------------------------------------------------------------
 // Issued by one elected lane of a converged warp: the warp-uniform operands stay in uniform registers (inside an
 // `if (lane == 0)` each MMA cost about 130 cycles of moving them there, 4 times its own time).
@@ -716,29 +716,9 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t smem_addr) {
 constexpr uint32_t kTcIdesc = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kTcIdescBMn = kTcIdesc | (1u << 16);  // B is MN-major
 
-// A wait that gives up after a number of polls (seconds; a healthy wait takes microseconds). Each poll may sleep in
-// hardware for a while (the hint), so the warps that wait leave the issue slots to the others: without it a tile
-// took 5900 cycles instead of 5100. A role that gave up ends its loop; the others then run into the same
-// limit in their next wait.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity) {
-#pragma unroll 1
-    for (int i = 0; i < (1 << 22); ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(100000)
-            : "memory");
-        if (ok) return true;
-    }
-    raise_fault(WZYB_FAULT_WAIT_TIMEOUT);
-    return false;
-}
 // by a whole warp, which goes on together
 __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, tc_wait(bar, parity));
+    return __all_sync(0xffffffffu, mbar_wait_asleep(bar, parity));
 }
 
 // the n lowest bits (none for n <= 0, all for n >= 32)
