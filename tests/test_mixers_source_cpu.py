@@ -42,3 +42,14 @@ def test_tensor_memory_changes_hands_between_fences():
     assert "tc_wait_st(); tc_fence_before(); warp_arrive(&sm.p_full[g / 2], lane);" in loop
     for wait in re.findall(r"tc_wait_warp\(&sm\.(?:s|x|o)_full[^;]*; if \(!ok\) break; (.{16})", loop):
         assert wait == "tc_fence_after()"
+
+
+def test_scan_stops_copying_after_a_lost_wait():
+    """A chunk's copies that did not arrive in time: the fetching warp starts no more copies into the buffers and waits
+    (bounded) for those in flight before the block's shared memory goes."""
+    text = re.sub(r"\s+", " ", source("gdn_delta.cu"))
+    fetch = text[text.index("if (role == 2) {"):text.index("if (role == 1) {")]
+    assert "if (lost < 0 && !mbar_wait(&full[(ch - 1) & 1], ((ch - 1) >> 1) & 1)) lost = ch - 1;" in fetch
+    assert fetch.count("bulk_load(") == 2 and fetch.index("if (lane == 0 && lost < 0) {") < fetch.index("bulk_load(")
+    end = fetch[fetch.index("cp_async_commit();"):]
+    assert "if (lost >= 0) mbar_wait_until(&full[lost & 1], (lost >> 1) & 1, globaltimer_ns() + kWaitLimitNs); return;" in end

@@ -682,11 +682,11 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
     constexpr int kBarReady = 1, kBarFree = 2, kBarHand = 3, kBarTaken = 7;
     if (role == 2) {
         const uint64_t policy = policy_evict_normal();
-        bool ok = true;  // a wait for a chunk that gave up is not repeated
+        int lost = -1;  // the chunk whose wait gave up: no wait and no copy follows, the results are void (and reported)
         for (int ch = 0; ch <= chunks; ++ch) {  // chunk ch is fetched while ch - 1 is worked through
             if (ch > 0) {
                 cp_async_wait<0>();
-                ok = ok && mbar_wait(&full[(ch - 1) & 1], ((ch - 1) >> 1) & 1);
+                if (lost < 0 && !mbar_wait(&full[(ch - 1) & 1], ((ch - 1) >> 1) & 1)) lost = ch - 1;
                 named_bar_sync(kBarReady, 160);  // chunk ch - 1 is there for the state warps
                 // the output warps have begun chunk ch - 1, so nobody reads chunk ch - 2's buffers any more; the state
                 // warps are past the products that the copies would slow down
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
             }
             if (ch == chunks) break;
             Stage& s = st[ch & 1];
-            if (lane == 0) {
+            if (lane == 0 && lost < 0) {
                 constexpr int kKq = sizeof(GdnKq<kSplit, HD>), kData = sizeof(GdnChunkData<kSplit>);
                 mbar_arrive_expect_tx(&full[ch & 1], kKq + kData);
                 bulk_load(&s.kq, p.kq + ((int64_t)ch * a.k_heads + hk) * kKq, kKq, &full[ch & 1], policy);
@@ -714,6 +714,8 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
             }
             cp_async_commit();
         }
+        // that chunk's copies are the only ones that can still be in flight
+        if (lost >= 0) mbar_wait_until(&full[lost & 1], (lost >> 1) & 1, globaltimer_ns() + kWaitLimitNs);
         return;
     }
     const int col = c0 + pair * 8 + 2 * t4;  // this lane's columns col, col + 1
