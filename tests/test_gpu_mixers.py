@@ -510,3 +510,59 @@ def test_attn_long_context_sums_do_not_drift(wz, dtype):
     at = [0, 7, T - 1]
     want = ref.attention(q[at], planes, kvh, hd, hd**-0.5, [list(range(n - T + t + 1)) for t in at])
     check_attention(q[at], out[at], lse[at], want)
+
+
+# ---- sizes of the factors of the delta rule ------------------------------------------------------
+
+
+def gdn_call(wz, q, k, v, g, beta, s0, **kw):
+    T, kh, hd = q.shape
+    vh = v.shape[1]
+    o, out = torch.full_like(v, 9.0, memory_format=torch.contiguous_format), torch.full((vh, hd, hd), 9.0, device=DEV)
+    wz.gdn_delta_rule(q, k, v, g, beta, o, out, state_in=s0, workspace=gdn_workspace(wz, T, kh, vh, hd), **kw)
+    return o, out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T", [50, 200])
+@pytest.mark.parametrize("by", ["scale", "q"])
+@pytest.mark.parametrize("down", [12, 20])
+def test_gdn_outputs_follow_small_queries_and_scales(wz, dtype, hd, T, by, down):
+    """o is linear in scale * q. A power of two there moves exponents only, so the outputs' bits stay the same (where they
+    are normal numbers) whatever the size, and hold the bounds of the recurrence at that size."""
+    r = gen(13)
+    q, k, v, g, beta, s0 = gdn_inputs(T, 2, 4, hd, torch.float32, r, False, False)
+    # q's elements are multiples of 2^-4, so that 2^-20 of them is exact in fp16 as well
+    q, k, v = (torch.round(16 * q) / 16).to(dtype), k.to(dtype), (512 * v).to(dtype)
+    s0 = 512 * s0
+    scale, f = hd**-0.5, 2.0**-down
+    assert torch.equal((q * f).to(dtype).double(), q.double() * f)
+    o1, s1 = gdn_call(wz, q, k, v, g, beta, s0, scale=scale, qk_l2norm=False)
+    o2, s2 = gdn_call(wz, q * f if by == "q" else q, k, v, g, beta, s0, scale=scale * (f if by == "scale" else 1), qk_l2norm=False)
+    want_o, want_s, snaps = ref.delta_rule(q, k, v, g, beta, s0, scale * f, None)
+    big = max(float(x.abs().max()) for x in snaps + [s0.double()]) + float(v.abs().max())
+    tol = big * ((T + 64) * 2.0**-22)
+    assert torch.equal(s1, s2) and (s2.double() - want_s).abs().max() <= tol
+    unit = 2.0**-10 if dtype == torch.float16 else 0.0
+    bound = unit * want_o.abs() + scale * f * (float(q.double().abs().sum(-1).max()) * tol + 2 * unit * big) + (2.0**-25 if unit else 0.0)
+    assert ((o2.double() - want_o).abs() <= bound).all()
+    # where the smaller output is a normal number before its rounding (2^-14 itself may have been rounded up to)
+    normal = o1.double().abs() * f > (2.0**-14 if dtype == torch.float16 else 2.0**-126)
+    assert normal.any() or (dtype == torch.float16 and down == 20)
+    assert torch.equal(o2.double()[normal], (o1.double() * f)[normal])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [50, 200])
+@pytest.mark.parametrize("down", [12, 30])
+def test_gdn_small_betas(wz, dtype, T, down):
+    """From an empty state every step adds beta (v - S k) k^T: with small betas throughout, a state of their size, whose
+    error is bounded by its own magnitude and that of beta v (two roundings at 2^-22 of either per step)."""
+    r = gen(14)
+    q, k, v, g, beta, _ = gdn_inputs(T, 2, 4, 128, dtype, r, False, True)
+    beta = beta * 2.0**-down
+    want_o, want_s, snaps = ref.delta_rule(q, k, v, g, beta, None, 128**-0.5, 1e-6)
+    big = max(float(x.abs().max()) for x in snaps) + float((beta.double().unsqueeze(-1) * v.double()).abs().max())
+    _, s = gdn_call(wz, q, k, v, g, beta, None)
+    assert (s.double() - want_s).abs().max() <= big * (T + 64) * 2.0**-22

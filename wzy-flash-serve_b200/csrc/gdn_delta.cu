@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             }
         }
         __syncthreads();
-        // T diag(beta) and P as fragments, scaled down only where they pass fp16's range
+        // T diag(beta) and P as fragments, their largest element scaled to [2^13, 2^14): the bits that fp16 parts hold do
+        // not depend on the sizes of beta, of the caller's scale or of an unnormed q
         float tv[8][4];
         float t_max = 0.f;
 #pragma unroll
@@ -526,9 +527,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             atomicMax(&sm.amax[1], pb);
         }
         __syncthreads();
-        int et = gdn_exp(__uint_as_float(sm.amax[0])) - 14, ep = gdn_exp(__uint_as_float(sm.amax[1])) - 14;
-        et = et < 0 ? 0 : et;
-        ep = ep < 0 ? 0 : ep;
+        const int et = gdn_exp(__uint_as_float(sm.amax[0])) - 14, ep = gdn_exp(__uint_as_float(sm.amax[1])) - 14;
         const float td = gdn_exp2i(-et), pd = gdn_exp2i(-ep);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
