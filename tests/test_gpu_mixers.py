@@ -566,3 +566,27 @@ def test_gdn_small_betas(wz, dtype, T, down):
     big = max(float(x.abs().max()) for x in snaps) + float((beta.double().unsqueeze(-1) * v.double()).abs().max())
     _, s = gdn_call(wz, q, k, v, g, beta, None)
     assert (s.double() - want_s).abs().max() <= big * (T + 64) * 2.0**-22
+
+
+# ---- uneven queries and keys ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("T", [1, 7, 40])
+@pytest.mark.parametrize("up", [0, 6, 12])
+def test_attn_uneven_groups(wz, dtype, hd, T, up):
+    """A query whose first group is 2^up times the others, over keys whose first group is 2^-up of theirs: all groups have
+    their share of the score, so none may lose bits beside the largest. 1, 7 and 40 tokens of 4 heads: both kernels."""
+    r = gen(21)
+    n = 300
+    rows, plane, desc = make_cache(wz, n, 16, n, hd, r, True)
+    for x in (rows[1], plane[1]):
+        x.view(torch.float16)[:, 0] *= 2.0**-up
+    q = torch.randn(T, 4, hd, generator=r, device=DEV)
+    q[:, :, :64] *= 2.0**up
+    q = q.to(dtype)
+    out, lse = torch.zeros_like(q), torch.zeros(T, 4, device=DEV)
+    wz.kv_attn(q, out, desc, 1, n, source=wz.KV_FULL, pos_offset=n - T, lse=lse, workspace=workspace(wz, T, 4, 1, hd))
+    see = [list(range(n - T + t + 1)) for t in range(T)]
+    check_attention(q, out, lse, ref.attention(q, rows, 1, hd, hd**-0.5, see))

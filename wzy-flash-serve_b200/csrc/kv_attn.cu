@@ -14,8 +14,8 @@
 // scale among the cells that the row sees, as the running maximum of its scores), so they sit in fp16's
 // upper range whatever the scales' size, and a row's result does not depend on cells it does not see. A
 // row's running maximum moves only when a score passes it by 2^8: its weights stay below 2^15 either way.
-// The second part of an fp32 call's weight enters 2^11 times as large and its products come back by 2^-11,
-// so that it is not cut off at fp16's smallest number.
+// The second part of an fp32 call's weight or query element enters 2^11 times as large and its products come back by
+// 2^-11, so that it is not cut off at fp16's smallest number.
 #include <type_traits>
 
 #include "launch.hpp"
@@ -233,7 +233,8 @@ __device__ __forceinline__ float exp2_int(int e) {  // 2^e, 0 below the normal r
 }
 
 // Query rows of a tile to shared memory as fp16 (kSplit: two parts of x * 2^-e, e from the row's largest
-// magnitude, so every fp32 row uses fp16's range). One warp per row in turn. qs[row * ld + col]; the
+// magnitude, so every fp32 row uses fp16's range; the second part 2^11 times as large, so that elements far below
+// the largest, which meet groups with large scales, keep their bits). One warp per row in turn. qs[row * ld + col]; the
 // factor that turns a raw dot into log2 units goes to row_scale.
 template <typename T, int HD, bool kSplit>
 __device__ __forceinline__ void stage_rows(const KvAttnArgs& a, int head, int row0, int rows, int ntile, __half* qs,
@@ -268,7 +269,7 @@ __device__ __forceinline__ void stage_rows(const KvAttnArgs& a, int head, int ro
         for (int i = 0; i < kE; ++i) {
             const __half h = __float2half_rn(x[i]);
             qs[r * ld + lane * kE + i] = h;
-            if constexpr (kSplit) ql[r * ld + lane * kE + i] = __float2half_rn(x[i] - __half2float(h));
+            if constexpr (kSplit) ql[r * ld + lane * kE + i] = __float2half_rn((x[i] - __half2float(h)) * kLoUp);
         }
         if (lane == 0) row_scale[r] = f;
     }
@@ -412,6 +413,7 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            [[maybe_unused]] float low[4] = {0.f, 0.f, 0.f, 0.f};
             const uint32_t w0[4] = {kr[0][n].x, kr[0][n].y, kr[0][n].z, kr[0][n].w};
             const uint32_t w1[4] = {kr[1][n].x, kr[1][n].y, kr[1][n].z, kr[1][n].w};
             const uint4 q0 = *reinterpret_cast<const uint4*>(qs + g * kLd + n * 64 + t4 * 16);
@@ -430,7 +432,11 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
                 const uint32_t fa[4] = {codes_f16(x0, kSelLo), codes_f16(x1, kSelLo), codes_f16(x0, kSelHi),
                                         codes_f16(x1, kSelHi)};
                 mma_f16(acc, fa, qb[2 * j], qb[2 * j + 1]);
-                if constexpr (kSplit) mma_f16(acc, fa, qc[2 * j], qc[2 * j + 1]);
+                if constexpr (kSplit) mma_f16(low, fa, qc[2 * j], qc[2 * j + 1]);
+            }
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] = fmaf(low[c], 1.f / kLoUp, acc[c]);
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[c] = fmaf(acc[c], ks[c >> 1][n], s[c]);
@@ -663,6 +669,13 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         : "memory");
 }
 // d = a * b + d * 2^-11
+__device__ __forceinline__ void tc_mma_ss_down11(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, 1, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %4, %4, %4}, p, 11;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(0)
+        : "memory");
+}
 __device__ __forceinline__ void tc_mma_ts_down11(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, 1, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
@@ -798,7 +811,8 @@ __global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile
     }
     if (warp < kSW) {
         // Query rows to shared memory, a lane 8 elements, several rows of a warp in flight. fp32
-        // rows enter as two fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range.
+        // rows enter as two fp16 parts of x * 2^-e, e from the row's largest magnitude, so they use fp16's range; the
+        // second part 2^11 times as large.
         constexpr int kL = HD / 8, kPer = 32 / kL, kRowsQ = S::kRows / kSW, kMineQ = kRowsQ / kPer;  // lanes per row, rows
         constexpr int kMostQ = kSplit ? 4 : 8, kBatch = kMineQ < kMostQ ? kMineQ : kMostQ;          // at a time, ...
         const int col = (lane % kL) * 8, g = col / 64, c16 = (col % 64) / 8;
@@ -835,12 +849,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile
                     const float down = exp2_int(-e);
                     uint32_t h[4], l[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x0 = x[2 * i] * down, x1 = x[2 * i + 1] * down;
-                        h[i] = pack_f16(x0, x1);
-                        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-                        l[i] = pack_f16(x0 - y.x, x1 - y.y);
-                    }
+                    for (int i = 0; i < 4; ++i) split_f16(x[2 * i] * down, x[2 * i + 1] * down, h[i], l[i]);
                     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[0][g]) + at) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sm.q[kSplit][g]) + at) = make_uint4(l[0], l[1], l[2], l[3]);
                     if (col == 0) sm.row_up[r] = exp2_int(e);
@@ -1242,14 +1251,17 @@ __global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile
                 tc_fence_after();
 #pragma unroll 1
                 for (int g = 0; g < NG; ++g) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        tc_mma_ss(tmem + g * 64, qd + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, x > 0);
-                    if constexpr (kSplit) {
+                    if constexpr (kSplit) {  // the second parts first: they come back by 2^-11 as the first ones are added
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            tc_mma_ss(tmem + g * 64, ql + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, 1);
+                            tc_mma_ss(tmem + g * 64, ql + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, x > 0);
+                        tc_mma_ss_down11(tmem + g * 64, qd + g * kQG, kd + g * kKG, kTcIdesc);
+                    } else {
+                        tc_mma_ss(tmem + g * 64, qd + g * kQG, kd + g * kKG, kTcIdesc, 0);
                     }
+#pragma unroll
+                    for (int x = 1; x < 4; ++x)
+                        tc_mma_ss(tmem + g * 64, qd + g * kQG + x * 2, kd + g * kKG + x * 2, kTcIdesc, 1);
                     if (g % 2 == 1 || g == NG - 1) tc_commit(&sm.s_full[g / 2]);
                 }
                 ok = tc_wait_warp(&sm.v_full, b);
