@@ -590,3 +590,18 @@ def test_attn_uneven_groups(wz, dtype, hd, T, up):
     wz.kv_attn(q, out, desc, 1, n, source=wz.KV_FULL, pos_offset=n - T, lse=lse, workspace=workspace(wz, T, 4, 1, hd))
     see = [list(range(n - T + t + 1)) for t in range(T)]
     check_attention(q, out, lse, ref.attention(q, rows, 1, hd, hd**-0.5, see))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 20, 40])
+@pytest.mark.parametrize("base", [2**30 - 21, 2**31 - 21, 2**31 + 5, 2**40])
+@pytest.mark.parametrize("window,sinks,seen", [(2**62, 0, 40), (7, 3, 3), (0, 2**40, 40), (9, 0, 0)])
+def test_attn_positions_past_31_bits(wz, dtype, T, base, window, sinks, seen):
+    """Queries that stand far past a short cache's end see its cells by the same rule."""
+    r = gen(22)
+    hd, n = 64, 40
+    rows, plane, desc = make_cache(wz, n, 16, n, hd, r, True)
+    q = torch.randn(T, 8, hd, generator=r, device=DEV).to(dtype)
+    out, lse = torch.ones_like(q), torch.zeros(T, 8, device=DEV)
+    wz.kv_attn(q, out, desc, 1, window, sinks, source=wz.KV_FULL, pos_offset=base, lse=lse, workspace=workspace(wz, T, 8, 1, hd))
+    check_attention(q, out, lse, ref.attention(q, rows, 1, hd, hd**-0.5, [list(range(seen))] * T))

@@ -62,9 +62,10 @@ struct KeyPlan {
     int sinks;
 };
 
-__device__ __forceinline__ int clamp_i32(int64_t x, int lo) {
-    return (int)(x < lo ? lo : (x > 0x7FFFFFFF ? 0x7FFFFFFF : x));
-}
+// Positions and cells are ints. No cell lies at this one or past it, so a query's own position may be cut to it, and
+// sums with a tile's size stay in range.
+constexpr int kMaxPos = 0x40000000;
+__device__ __forceinline__ int clamp_pos(int64_t x) { return (int)(x < -1 ? -1 : (x > kMaxPos ? kMaxPos : x)); }
 
 // A row sees positions j with j <= hi and (j < sinks or j > lo).
 struct RowSpan {
@@ -73,8 +74,8 @@ struct RowSpan {
 __device__ __forceinline__ RowSpan row_span(const KvAttnArgs& a, int64_t base, int t) {
     const int64_t p = base + (a.tree ? (int64_t)__ldg(a.depth + t) : t);
     RowSpan r;
-    r.hi = clamp_i32(p, -1);
-    r.lo = clamp_i32(p - a.window, -1);
+    r.hi = clamp_pos(p);
+    r.lo = clamp_pos(p - a.window);
     return r;
 }
 
@@ -1507,7 +1508,6 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     if (tree && (!drafts || !mask || !depth || !drafts->ring_k_q || !drafts->ring_k_s || !drafts->ring_v_q ||
                  !drafts->ring_v_s))
         return WZYB_ERR_NULL;
-    constexpr int64_t kMaxPos = 0x40000000;  // positions and cells are ints, with room for a tile past them
     if (T_ < 0 || T_ > (1 << 22) || x.kv_heads < 1 || x.kv_heads > 64 || x.q_heads < 1 || x.q_heads > 256 ||
         x.q_heads % x.kv_heads != 0 || (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) ||
         x.window < 0 || x.sinks < 0 || c.max_ctx < 0 || c.max_ctx > kMaxPos ||
@@ -1557,7 +1557,7 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     a.kv_heads = x.kv_heads;
     a.d_base_pos = x.d_base_pos;
     a.pos_offset = x.pos_offset;
-    a.window = x.window < (int64_t(1) << 40) ? x.window : (int64_t(1) << 40);
+    a.window = x.window < (int64_t(1) << 62) ? x.window : (int64_t(1) << 62);  // p - window stays in range
     a.sinks = x.sinks;
     a.scale_log2 = x.scale * kLog2e;
     a.ring_div = full ? 1 : (uint64_t)(c.ring_cap <= 2 * kKvSinkPin ? c.ring_cap : c.ring_cap - kKvSinkPin);
