@@ -149,3 +149,12 @@ def test_wrappers_refuse_wrong_tensors(wz):
         wz.kv_attn(q.to(torch.bfloat16), q, c, 1, 16)
     with pytest.raises(ValueError):
         wz.gdn_delta_rule(q, q, q, None, None, q, None)
+
+
+@pytest.mark.parametrize("fn", ["wzyb_kv_attn_f16", "wzyb_kv_attn_f32"])
+def test_attn_refuses_a_misaligned_base_position(wz, fn):
+    """The kernels read it as one 4-byte word."""
+    f = getattr(wz.lib(), fn)
+    for at in (1, 2, 3):
+        assert f(ctypes.byref(attn_args(wz, cache(wz), d_base_pos=A16 + at)), 0, None) == wz.ERR_ALIGN
+    assert f(ctypes.byref(attn_args(wz, cache(wz), d_base_pos=A16 + 4)), 0, None) == wz.OK

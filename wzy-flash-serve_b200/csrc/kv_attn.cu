@@ -1521,7 +1521,7 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     if (!aligned16(x.q) || !aligned16(x.out) || ((x.q_head_stride * kB) % 16) != 0 || ((x.q_row_stride * kB) % 16) != 0 ||
         ((x.out_head_stride * kB) % 16) != 0 || ((x.out_row_stride * kB) % 16) != 0 || !planes_aligned(c, full) ||
         (tree && !planes_aligned(*drafts, false)) || ((uintptr_t)x.lse & 3) != 0 || ((uintptr_t)mask & 3) != 0 ||
-        ((uintptr_t)depth & 3) != 0)
+        ((uintptr_t)depth & 3) != 0 || ((uintptr_t)x.d_base_pos & 3) != 0)
         return WZYB_ERR_ALIGN;
     if (T_ == 0) return WZYB_OK;
     // the most keys that a row tile can see, as far as the host knows
