@@ -487,7 +487,8 @@ int wzyb_embed_ple_f16(const wzyb_embed_ple_args* a, int64_t T, wzyb_stream_t st
  *   x_j = scale * (q . k_j);  out = sum_j softmax(x)_j v_j;  lse[t, h] = ln sum_j exp(x_j)  (lse may be NULL)
  * with k_j, v_j = code * scale of the cell's 64-element groups. A query that sees nothing gets out = 0 and
  * lse = -inf. Cells that a query does not see never reach its result, whatever they hold.
- * head_dim in {64, 128, 256}; q_heads a multiple of kv_heads, at most 256; kv_heads <= 64; T <= 2^22;
+ * head_dim in {64, 128, 256}; q_heads a multiple of kv_heads, at most 256; kv_heads <= 64; T <= 2^22 (0: nothing to
+ * do, the per-token pointers may be NULL);
  * max_ctx and ring_cap at most 2^30; strides in elements. Cache codes and scales 16-byte aligned.
  * workspace: wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim) bytes of device memory (0: none needed),
  * 16-byte aligned, of no meaning between calls; calls on different streams need their own.

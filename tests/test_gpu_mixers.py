@@ -605,3 +605,13 @@ def test_attn_positions_past_31_bits(wz, dtype, T, base, window, sinks, seen):
     out, lse = torch.ones_like(q), torch.zeros(T, 8, device=DEV)
     wz.kv_attn(q, out, desc, 1, window, sinks, source=wz.KV_FULL, pos_offset=base, lse=lse, workspace=workspace(wz, T, 8, 1, hd))
     check_attention(q, out, lse, ref.attention(q, rows, 1, hd, hd**-0.5, [list(range(seen))] * T))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attn_no_tokens(wz, dtype):
+    """Empty tensors through the bindings."""
+    _, _, desc = make_cache(wz, 10, 16, 100, 64, gen(23), False)
+    q = torch.empty(0, 4, 64, dtype=dtype, device=DEV)
+    wz.kv_attn(q, torch.empty_like(q), desc, 1, 16, lse=torch.empty(0, 4, device=DEV))
+    wz.kv_tree_attn(q, torch.empty_like(q), desc, desc, torch.empty(0, 0, dtype=torch.int32, device=DEV), 1, 16,
+                    torch.empty(0, dtype=torch.int32, device=DEV))

@@ -158,3 +158,15 @@ def test_attn_refuses_a_misaligned_base_position(wz, fn):
     for at in (1, 2, 3):
         assert f(ctypes.byref(attn_args(wz, cache(wz), d_base_pos=A16 + at)), 0, None) == wz.ERR_ALIGN
     assert f(ctypes.byref(attn_args(wz, cache(wz), d_base_pos=A16 + 4)), 0, None) == wz.OK
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attn_no_tokens(wz, dtype):
+    """No tokens are no work: an empty tensor has a null pointer, which is then no error (as in the delta rule)."""
+    c, d = cache(wz), cache(wz, ring_cap=8)
+    a = attn_args(wz, c, q=None, out=None, workspace=None, workspace_bytes=0)
+    assert getattr(wz.lib(), f"wzyb_kv_attn_{dtype}")(ctypes.byref(a), 0, None) == wz.OK
+    assert getattr(wz.lib(), f"wzyb_kv_tree_attn_{dtype}")(ctypes.byref(a), ctypes.byref(d), None, None, 0, None) == wz.OK
+    empty = wz.kv_cache(*(torch.empty(0) for _ in range(4)), 0, 0)
+    assert getattr(wz.lib(), f"wzyb_kv_tree_attn_{dtype}")(ctypes.byref(a), ctypes.byref(empty), None, None, 0, None) == wz.OK
+    assert getattr(wz.lib(), f"wzyb_kv_attn_{dtype}")(ctypes.byref(attn_args(wz, c, q=None)), 1, None) == wz.ERR_NULL

@@ -1501,12 +1501,12 @@ static int attn_entry(const wzyb_kv_attn_args* p, const wzyb_kv_cache* drafts, c
     const wzyb_kv_cache& c = *x.cache;
     if (x.source != WZYB_KV_RING && x.source != WZYB_KV_FULL) return WZYB_ERR_VALUE;
     const bool full = x.source == WZYB_KV_FULL;
-    if (!x.q || !x.out) return WZYB_ERR_NULL;
+    if (T_ != 0 && (!x.q || !x.out)) return WZYB_ERR_NULL;
     if (full ? !(c.full_k_q && c.full_k_s && c.full_v_q && c.full_v_s)
              : !(c.ring_k_q && c.ring_k_s && c.ring_v_q && c.ring_v_s))
         return WZYB_ERR_NULL;
-    if (tree && (!drafts || !mask || !depth || !drafts->ring_k_q || !drafts->ring_k_s || !drafts->ring_v_q ||
-                 !drafts->ring_v_s))
+    if (tree && (!drafts || (T_ != 0 && (!mask || !depth || !drafts->ring_k_q || !drafts->ring_k_s || !drafts->ring_v_q ||
+                                         !drafts->ring_v_s))))
         return WZYB_ERR_NULL;
     if (T_ < 0 || T_ > (1 << 22) || x.kv_heads < 1 || x.kv_heads > 64 || x.q_heads < 1 || x.q_heads > 256 ||
         x.q_heads % x.kv_heads != 0 || (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) ||
