@@ -491,7 +491,8 @@ int wzyb_embed_ple_f16(const wzyb_embed_ple_args* a, int64_t T, wzyb_stream_t st
  * do, the per-token pointers may be NULL);
  * max_ctx and ring_cap at most 2^30; strides in elements. Cache codes and scales 16-byte aligned.
  * workspace: wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim) bytes of device memory (0: none needed),
- * 16-byte aligned, of no meaning between calls; calls on different streams need their own.
+ * 16-byte aligned, of no meaning between calls; calls on different streams need their own. The size does not grow
+ * with T (long calls need none): 18944 * (4 * head_dim + 8) + 16 bytes serve every T and every head count.
  * ========================================================================================== */
 #define WZYB_KV_RING 0
 #define WZYB_KV_FULL 1
@@ -546,7 +547,7 @@ int wzyb_kv_tree_attn_f32(const wzyb_kv_attn_args* a, const wzyb_kv_cache* draft
  * head_dim] or NULL: the state after every token, for taking back rejected drafts. head_dim in {64, 128};
  * v_heads a multiple of k_heads, at most 1024; T = 0 copies the state. o must not overlap the inputs.
  * workspace: wzyb_gdn_delta_rule_workspace(T, k_heads, v_heads, head_dim) bytes of device memory (0: none),
- * 16-byte aligned, of no meaning between calls.
+ * 16-byte aligned, of no meaning between calls; one for the largest T serves the shorter calls (96 MiB at most).
  * ========================================================================================== */
 typedef struct {
     const void* q;

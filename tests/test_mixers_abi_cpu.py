@@ -170,3 +170,22 @@ def test_attn_no_tokens(wz, dtype):
     empty = wz.kv_cache(*(torch.empty(0) for _ in range(4)), 0, 0)
     assert getattr(wz.lib(), f"wzyb_kv_tree_attn_{dtype}")(ctypes.byref(a), ctypes.byref(empty), None, None, 0, None) == wz.OK
     assert getattr(wz.lib(), f"wzyb_kv_attn_{dtype}")(ctypes.byref(attn_args(wz, c, q=None)), 1, None) == wz.ERR_NULL
+
+
+@pytest.mark.parametrize("kh,vh,hd", [(16, 32, 128), (16, 48, 128), (2, 6, 64), (1, 1024, 128), (1024, 1024, 128)])
+def test_delta_rule_workspace_of_the_largest_call_serves_shorter_ones(wz, kh, vh, hd):
+    sizes = [wz.gdn_delta_rule_workspace_bytes(T, kh, vh, hd) for T in list(range(1, 4000, 7)) + list(range(4000, 70000, 333))]
+    assert sizes == sorted(sizes)
+    assert sizes[-1] <= 96 << 20
+
+
+def test_attn_workspace_bound_for_every_length(wz):
+    """The one size that the header gives for all calls."""
+    worst = 0
+    for qh, kvh in [(16, 2), (24, 2), (8, 2), (6, 1), (3, 3), (64, 64), (256, 1), (256, 64), (1, 1), (7, 7)]:
+        for T in list(range(1, 700)) + list(range(700, 9000, 37)):
+            for hd in (64, 256):
+                n = wz.kv_attn_workspace_bytes(T, qh, kvh, hd)
+                assert n <= 18944 * (4 * hd + 8) + 16, (T, qh, kvh, hd)
+            worst = max(worst, n)
+    assert worst > 18000 * (4 * 256 + 8)  # and it is not a loose one

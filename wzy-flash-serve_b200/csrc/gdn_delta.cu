@@ -907,10 +907,15 @@ static int64_t gdn_chunk_bytes(bool f32, int k_heads, int v_heads, int head_dim)
     return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * 2 * row
                : v_heads * (int64_t)sizeof(GdnChunkData<false>) + k_heads * row;
 }
-static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
+static int64_t gdn_most_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
     const int64_t n = kGdnSegBytes / gdn_chunk_bytes(f32, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
-    const int64_t segs = n < 1 ? all : (all + n - 1) / n;
-    return segs < 1 ? 1 : (all + segs - 1) / segs;  // segments of one size: a short last one costs as much as a long one's start
+    return n < 1 ? 1 : (all < n ? all : n);
+}
+// Chunks per segment, at most that many: segments of one size, as a short last one costs as much as a long one's start.
+static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
+    const int64_t most = gdn_most_chunks(f32, T, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
+    const int64_t segs = (all + most - 1) / most;
+    return (all + segs - 1) / segs;
 }
 // Calls of at least this many tokens take the chunked form. Chunked / token by token, us per call: fp16 16/32 heads of
 // 128, 64 tokens 22 / 21, 96 26 / 30, 256 34 / 78; fp32 16/48 heads 64 tokens 38 / 32, 96 45 / 47; fp32 2/6 heads of
@@ -1011,7 +1016,7 @@ int64_t wzyb_gdn_delta_rule_workspace(int64_t T, int k_heads, int v_heads, int h
     if (T < wzyb::kGdnChunkedFrom || k_heads < 1 || v_heads < 1 || head_dim < 1) return 0;
     int64_t most = 0;
     for (int f32 = 0; f32 < 2; ++f32) {
-        const int64_t bytes = wzyb::gdn_seg_chunks(f32 != 0, T, k_heads, v_heads, head_dim) *
+        const int64_t bytes = wzyb::gdn_most_chunks(f32 != 0, T, k_heads, v_heads, head_dim) *
                               wzyb::gdn_chunk_bytes(f32 != 0, k_heads, v_heads, head_dim);
         most = bytes > most ? bytes : most;
     }
