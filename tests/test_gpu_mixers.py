@@ -615,3 +615,113 @@ def test_attn_no_tokens(wz, dtype):
     wz.kv_attn(q, torch.empty_like(q), desc, 1, 16, lse=torch.empty(0, 4, device=DEV))
     wz.kv_tree_attn(q, torch.empty_like(q), desc, desc, torch.empty(0, 0, dtype=torch.int32, device=DEV), 1, 16,
                     torch.empty(0, dtype=torch.int32, device=DEV))
+
+
+# ---- rows beside cells that they do not see, scales ----------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [8, 40])  # both kernels
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 60000.0])
+def test_attn_earlier_rows_keep_their_bits(wz, dtype, T, bad):
+    """A cell that only the later rows see, with an infinite, a NaN or a 2^20-fold value scale: the earlier rows' weights are
+    scaled by what they see alone, so their bits stay; the later rows are spoiled, or right for the huge cell."""
+    n, hd, at = 40, 64, 36
+    r = gen(24)
+    rows, plane, desc = make_cache(wz, n, 16, n, hd, r, True)
+    q = torch.randn(T, 4, hd, generator=r, device=DEV).to(dtype)
+    base, ws = n - T, workspace(wz, T, 4, 1, hd)
+    outs = []
+    for scale in (1.0, bad):
+        rows[3].view(torch.float16)[at, 0] = plane[3].view(torch.float16)[at, 0] = scale
+        out, lse = torch.zeros_like(q), torch.zeros(T, 4, device=DEV)
+        wz.kv_attn(q, out, desc, 1, 100, source=wz.KV_FULL, pos_offset=base, lse=lse, workspace=ws)
+        outs.append((out, lse))
+    early = at - base
+    assert torch.equal(outs[0][0][:early], outs[1][0][:early]) and torch.equal(outs[0][1][:early], outs[1][1][:early])
+    if math.isfinite(bad):
+        see = [list(range(base + t + 1)) for t in range(T)]
+        if dtype == torch.float16:  # means of values up to 60000 * 127 pass fp16's range
+            assert torch.isinf(outs[1][0][early:]).any() or outs[1][0][early:].abs().max() > 1000
+        else:
+            check_attention(q, *outs[1], ref.attention(q, rows, 1, hd, hd**-0.5, see))
+    else:
+        assert not torch.isfinite(outs[1][0][early:]).any(-1).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [2, 40])
+@pytest.mark.parametrize("scale", [0.0, 1e-4, 0.3, -0.2])
+def test_attn_scale(wz, dtype, T, scale):
+    r = gen(25)
+    n, hd = 150, 128
+    rows, _, desc = make_cache(wz, n, 16, n, 2 * hd, r, True)
+    q = torch.randn(T, 8, hd, generator=r, device=DEV).to(dtype)
+    out, lse = torch.zeros_like(q), torch.zeros(T, 8, device=DEV)
+    wz.kv_attn(q, out, desc, 2, n, scale=scale, source=wz.KV_FULL, pos_offset=n - T, lse=lse, workspace=workspace(wz, T, 8, 2, hd))
+    o, wl, mag, _ = ref.attention(q, rows, 2, hd, scale, [list(range(n - T + t + 1)) for t in range(T)])
+    dot = torch.zeros_like(wl)  # the largest sum of |scale q k|, which a negative scale's maximum is not
+    for h in range(2):
+        k = ref.rows64(rows[0], rows[1], hd, h).abs()
+        dot[:, 4 * h:4 * h + 4] = abs(scale) * (q[:, 4 * h:4 * h + 4].double().abs() @ k.T).amax(-1)
+    check_attention(q, out, lse, (o, wl, mag, dot))
+
+
+# ---- the delta rule over many chunks and segments ------------------------------------------------
+
+
+def delta_rule_long(q, k, v, g, beta, state, scale):
+    """ref.delta_rule without keeping every state; also, per token, the largest |state| and the sum of the earlier steps'
+    shares in an error at it: a step's map shrinks an error by its decay at least."""
+    T, kh, d = q.shape
+    vh = v.shape[1]
+    q, k, v, beta, keep = q.double(), k.double(), v.double(), beta.double(), torch.exp(g.double())
+    q, k = (x / torch.sqrt((x * x).sum(-1, keepdim=True) + 1e-6) for x in (q, k))
+    q, k = (x.repeat_interleave(vh // kh, 1) for x in (q, k))
+    s, o, size = state.double().clone(), torch.zeros_like(v), torch.zeros(T, dtype=torch.float64, device=v.device)
+    eff, most = torch.zeros(vh, dtype=torch.float64, device=v.device), torch.zeros(vh, dtype=torch.float64, device=v.device)
+    for t in range(T):
+        s *= keep[t][:, None, None]
+        e = beta[t][:, None] * (v[t] - (s @ k[t].unsqueeze(-1)).squeeze(-1))
+        s += e[:, :, None] * k[t][:, None, :]
+        o[t] = scale * (s @ q[t].unsqueeze(-1)).squeeze(-1)
+        size[t] = s.abs().max()
+        eff = eff * keep[t] + 1
+        most = torch.maximum(most, eff)
+    return o, s, size, float(most.max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,kh,vh,hd", [(1100, 2, 4, 128), (2111, 2, 4, 64), (6037, 16, 32, 128), (3100, 16, 48, 128)])
+def test_gdn_many_chunks_and_segments(wz, dtype, T, kh, vh, hd):
+    """More than 16 chunks (the columns' exponents are set anew), and lengths that take two segments of the workspace in one
+    type or in both, the last one ragged; state in place, a workspace of the exact size with a guard behind it."""
+    r = gen(30 + T)
+    q, k, v, g, beta, s0 = gdn_inputs(T, kh, vh, hd, dtype, r, True, True)
+    want_o, want_s, size, eff = delta_rule_long(q, k, v, g, beta, s0, hd**-0.5)
+    need = wz.gdn_delta_rule_workspace_bytes(T, kh, vh, hd)
+    ws = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+    ws[:need] = 255
+    o, state = torch.full((T + 1, vh, hd), 9.0, dtype=dtype, device=DEV), s0.clone()
+    wz.gdn_delta_rule(q, k, v, g, beta, o[:T], state, state_in=state, workspace=ws[:need])
+    assert (ws[need:] == 0xA5).all() and (o[T] == 9).all()
+    big = float(max(size.max(), s0.abs().max()) + v.abs().max())
+    # check_gdn's bound with the steps that count under the decays in the place of all T
+    check_gdn(dtype, min(T, math.ceil(eff)), o[:T], state, want_o, want_s, big, hd**-0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [2111, 3200])
+def test_gdn_falling_magnitudes(wz, dtype, T):
+    """Values and states that shrink by 2^20 over the call: the columns' exponents follow them down every 16 chunks, so an
+    error is bounded by the magnitudes of the last 17 chunks, not by the call's largest."""
+    r = gen(31)
+    q, k, v, g, beta, s0 = gdn_inputs(T, 2, 4, 128, torch.float32, r, False, True)
+    fall = 2.0 ** (10 - 20 * torch.arange(T, device=DEV) / T)
+    q, k, v, s0 = q.to(dtype), k.to(dtype), (v * fall[:, None, None]).to(dtype), s0 * 2.0**10
+    want_o, want_s, size, eff = delta_rule_long(q, k, v, g, beta, s0, 128**-0.5)
+    o, state = torch.zeros_like(v), torch.zeros_like(s0)
+    wz.gdn_delta_rule(q, k, v, g, beta, o, state, state_in=s0, workspace=gdn_workspace(wz, T, 2, 4, 128))
+    late = slice(T - 17 * 64, T)
+    big = float(size[late].max() + v[late].abs().max())
+    assert (state.double() - want_s).abs().max() <= big * (math.ceil(eff) + 64) * 2.0**-22
