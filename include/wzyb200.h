@@ -545,7 +545,9 @@ int wzyb_kv_tree_attn_f32(const wzyb_kv_attn_args* a, const wzyb_kv_cache* draft
  * x * rsqrt(sum x^2 + l2_eps). state_in [v_heads, head_dim, head_dim] fp32 or NULL (zeros), state_out the
  * state after the last token (the same buffer as state_in is allowed); state_snaps [T, v_heads, head_dim,
  * head_dim] or NULL: the state after every token, for taking back rejected drafts. head_dim in {64, 128};
- * v_heads a multiple of k_heads, at most 1024; T = 0 copies the state. o must not overlap the inputs.
+ * v_heads a multiple of k_heads, at most 1024; T = 0 copies the state. o must not overlap the inputs. An infinite or
+ * NaN q spoils its token's outputs, a v its column and a k, g (but -inf) or beta its heads from its token on; no
+ * earlier token's.
  * workspace: wzyb_gdn_delta_rule_workspace(T, k_heads, v_heads, head_dim) bytes of device memory (0: none),
  * 16-byte aligned, of no meaning between calls; one for the largest T serves the shorter calls (96 MiB at most).
  * ========================================================================================== */

@@ -725,3 +725,33 @@ def test_gdn_falling_magnitudes(wz, dtype, T):
     late = slice(T - 17 * 64, T)
     big = float(size[late].max() + v[late].abs().max())
     assert (state.double() - want_s).abs().max() <= big * (math.ceil(eff) + 64) * 2.0**-22
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [60, 150])  # token by token, chunked
+@pytest.mark.parametrize("l2", [True, False])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta"])
+def test_gdn_infinities_and_nan_reach_no_earlier_token(wz, dtype, T, l2, bad, what):
+    """A q spoils its own token's outputs, a v its column from its token on, a k, g or beta its head from there on; all
+    other outputs and states keep their bits."""
+    if what == "g" and bad == -math.inf:
+        pytest.skip("a reset")
+    r = gen(26)
+    x = gdn_inputs(T, 2, 4, 128, dtype, r, False, l2)
+    names, at = ["q", "k", "v", "g", "beta", "s0"], T - 55
+    assert 0 < at % 64 < 63
+    clean = gdn_call(wz, *x, qk_l2norm=l2)
+    y = [t.clone() for t in x]
+    y[names.index(what)][(at, 1) if what in ("g", "beta") else (at, 1, 33)] = bad
+    o, s = gdn_call(wz, *y, qk_l2norm=l2)
+    spoiled_o, spoiled_s = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(s, dtype=torch.bool)
+    if what == "q":
+        spoiled_o[at, 2:] = True
+    elif what == "v":
+        spoiled_o[at:, 1, 33] = spoiled_s[1, 33] = True
+    else:
+        heads = slice(2, 4) if what == "k" else slice(1, 2)  # two value heads share a key head
+        spoiled_o[at:, heads] = spoiled_s[heads] = True
+    assert torch.equal(o[~spoiled_o], clean[0][~spoiled_o]) and torch.equal(s[~spoiled_s], clean[1][~spoiled_s])
+    assert not torch.isfinite(o[spoiled_o]).any() and not torch.isfinite(s[spoiled_s]).any()

@@ -206,9 +206,16 @@ __global__ void __launch_bounds__(256) gdn_recurrent_kernel(const GdnDeltaArgs a
 // calls are one part and exact. The exponents e are per value column (columns never mix), P and T have one each.
 // Running sums never live in a tensor-core accumulator for longer than a chunk (its sums are cut off towards
 // zero): S is updated in fp32 registers.
+//
+// Infinities and NaN. A masked product is 0 times a later token's value, which is no 0 where that is infinite or NaN,
+// and one such value would set the exponent of its whole column. So they are taken out: an infinite or NaN k, g
+// (not -inf) or beta ends the chunk's matrices before its token, an infinite or NaN element of X (from a v, or from a
+// state that is so already) is replaced by 0, and what follows from them (all later outputs and the state, of the head or
+// of the column) is set to NaN. A q reaches its own row only.
 // ----------------------------------------------------------------------------------------------------
 constexpr int kGdnChunk = 64;
 constexpr float kGdnLo = 2048.f;
+constexpr float kGdnFinite = 3.402823466e38f;  // the largest finite number: neither an infinity nor a NaN is <= it
 
 // A (chunk, value head)'s part of the workspace. Matrices as mma A fragments, 16 bytes per lane: fragment
 // (m-tile i, k-step j <= i) at index i * (i + 1) / 2 + j, 512 bytes each.
@@ -263,7 +270,29 @@ struct GdnPrepSmem {
     float tm[64][68];
     float rk[64], rq[64], beta[64], ghi[64], glo[64];
     unsigned int amax[2];
+    unsigned int k_bad[2];  // bit per token: k is infinite or NaN
+    int first_bad;          // of the value head: the first token from which everything is NaN, 64 for none
 };
+
+// The rows of k that hold an infinity or a NaN become 0 in the chunk's images; k_bad names them.
+template <typename T, int HD>
+__device__ __noinline__ void gdn_zero_bad_k(const GdnPrepArgs& p, GdnPrepSmem<T, HD>& sm, GdnKq<sizeof(T) == 4, HD>& image, int64_t tok0, int hk,
+                                            int n) {
+    constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+    bool bad = false;
+    const int r = threadIdx.x;
+    if (r < n) {
+        const T* const k = static_cast<const T*>(p.x.k) + (tok0 + r) * p.x.k_row + hk * HD;
+        for (int i = 0; i < HD; ++i) bad = bad || !(fabsf((float)k[i]) <= kGdnFinite);
+        for (int part = 0; bad && part < kParts; ++part)
+            for (int i = 0; i < HD; ++i) sm.kq.k[part][r * (HD + 8) + i] = image.k[part][r * (HD + 8) + i] = __float2half_rn(0.f);
+        if (bad) sm.rk[r] = 0.f;
+    }
+    const unsigned int bits = __ballot_sync(0xffffffffu, bad);
+    __syncthreads();
+    if (r < 64 && r % 32 == 0) sm.k_bad[r / 32] = bits;
+    __syncthreads();
+}
 
 // One CTA of 4 warps per (chunk, k head), over the value heads that share it. Warp w owns rows 16w .. 16w+15.
 // T by blocks of 16: a diagonal block's inverse by forward substitution (a lane per column), then the column
@@ -287,6 +316,8 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
     constexpr int kL = HD / 8;  // lanes per row
     GdnKq<kSplit, HD>& image = reinterpret_cast<GdnKq<kSplit, HD>*>(p.kq)[(int64_t)chunk * a.k_heads + hk];
 
+    if (tid < 2) sm.k_bad[tid] = 0u;
+    __syncthreads();
     for (int r0 = 0; r0 < 64; r0 += 128 / kL) {
         const int r = r0 + tid / kL, col = (tid % kL) * 8;
         float x[2][8];
@@ -307,6 +338,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
                 am = fmaxf(am, fabsf(x[m][i]));
             }
             ss = group_sum<kL>(ss);
+            if (m == 0 && col == 0 && !(ss <= kGdnFinite)) sm.k_bad[r >> 5] = 1u;  // infinite or NaN, or too large to be squared
             f[m] = r < n ? (a.l2norm ? rsqrtf(ss + a.l2_eps) : 1.f) : 0.f;
             __half* const hi = (m ? sm.kq.q[0] : sm.kq.k[0]) + r * kLd + col;
             if constexpr (kSplit) {
@@ -335,6 +367,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
         }
     }
     __syncthreads();
+    if ((sm.k_bad[0] | sm.k_bad[1]) != 0u) gdn_zero_bad_k<T, HD>(p, sm, image, tok0, hk, n);
 
     // raw k.k and q.k of this warp's rows, columns up to the diagonal block
     float kk[8][4], qk[8][4];
@@ -403,6 +436,18 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             // running sums in fp64, held as two fp32 parts in log2 units: differences of close tokens keep their
             // precision after strong decays. A decay below e^-120 is 0 in fp32 either way (so -inf is as well).
             double s0 = 0., s1 = 0.;
+            bool bad[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                bad[i] = !(gx[i] <= kGdnFinite) || !(fabsf(bx[i]) <= kGdnFinite) || (sm.k_bad[lane >> 4] >> ((2 * lane + i) & 31) & 1u);
+            int first = 64;
+            if (__any_sync(0xffffffffu, bad[0] || bad[1])) {
+                first = __reduce_min_sync(0xffffffffu, bad[0] ? 2 * lane : (bad[1] ? 2 * lane + 1 : 64));
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (2 * lane + i >= first) gx[i] = bx[i] = 0.f;
+            }
+            if (lane == 0) sm.first_bad = first;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 sm.beta[2 * lane + i] = bx[i];
@@ -442,7 +487,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
         if (tid < 64) {
             const float e = ex2_approx(sm.ghi[tid] + sm.glo[tid]);
             out.a[tid] = sm.rk[tid] * e;
-            out.b[tid] = sm.rq[tid] * e;
+            out.b[tid] = tid < sm.first_bad ? sm.rq[tid] * e : __int_as_float(0x7FC00000);
             out.c[tid] = sm.rk[tid] * ex2_approx((sm.ghi[63] - sm.ghi[tid]) + (sm.glo[63] - sm.glo[tid]));
         }
         __syncwarp();
@@ -520,6 +565,16 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
                 t_max = fmaxf(t_max, fabsf(tv[i][c]));
             }
         }
+        if (p_max > kGdnFinite) {  // an infinite q: its rows are alone with it
+            p_max = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i > 2 * warp + 1) break;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (fabsf(pv[i][c]) <= kGdnFinite) p_max = fmaxf(p_max, fabsf(pv[i][c]));
+            }
+        }
         const unsigned int tb = __reduce_max_sync(0xffffffffu, __float_as_uint(t_max));
         const unsigned int pb = __reduce_max_sync(0xffffffffu, __float_as_uint(p_max));
         if (lane == 0) {
@@ -550,7 +605,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
             if constexpr (kSplit) out.p[10 + at][lane] = make_uint4(l[0], l[1], l[2], l[3]);
         }
         if (tid == 0) {
-            out.decay = ex2_approx(sm.ghi[63] + sm.glo[63]);
+            out.decay = sm.first_bad < 64 ? __int_as_float(0x7FC00000) : ex2_approx(sm.ghi[63] + sm.glo[63]);
             out.t_up = gdn_exp2i(et);
             out.p_up = gdn_exp2i(ep);
             out.pad = 0.f;
@@ -578,7 +633,22 @@ struct GdnScanStage {
 
 // Two column exponents per lane (columns 2*t4, 2*t4 + 1 of its warp), alike over the lanes of a column: values
 // scaled by 2^-e stay below 2^14. `force` sets them anew (every 16 chunks, so they follow a shrinking state
-// down too); otherwise they move only when a value would pass 2^14.
+// down too); otherwise they move only when a value would pass 2^14. `m`: the lane's largest magnitudes.
+__device__ __forceinline__ bool gdn_exp_moves(const float (&m)[2], const int (&e)[2], bool force) {
+    const bool over = !(m[0] * gdn_exp2i(-e[0]) <= 16384.f) || !(m[1] * gdn_exp2i(-e[1]) <= 16384.f);
+    return __any_sync(0xffffffffu, over) || force;
+}
+__device__ __forceinline__ void gdn_move_exp(float (&m)[2], int (&e)[2], bool force) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+        if (force || m[i] * gdn_exp2i(-e[i]) > 16384.f) {
+            const int n = gdn_exp(m[i]) - 8;
+            e[i] = n < -100 ? -100 : n;
+        }
+    }
+}
 template <int N>
 __device__ __forceinline__ void gdn_col_exp(const float (&x)[N][4], int (&e)[2], bool force) {
     float m[2] = {0.f, 0.f};
@@ -586,18 +656,41 @@ __device__ __forceinline__ void gdn_col_exp(const float (&x)[N][4], int (&e)[2],
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) m[c & 1] = fmaxf(m[c & 1], fabsf(x[i][c]));
-    const bool over = m[0] * gdn_exp2i(-e[0]) > 16384.f || m[1] * gdn_exp2i(-e[1]) > 16384.f;
-    if (__any_sync(0xffffffffu, over) || force) {
+    if (gdn_exp_moves(m, e, force)) gdn_move_exp(m, e, force);
+}
+// The largest magnitude of three, NaN where one is.
+__device__ __forceinline__ float max3_abs_nan(float a, float x, float y) {
+    float z;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(z) : "f"(a), "f"(x), "f"(y));
+    return z;
+}
+// For X: also the first infinite or NaN row of each of the two columns (unchanged where there is none, which is to say
+// always); such elements become 0.
+__device__ __forceinline__ void gdn_clean_exp(float (&x)[4][4], int (&e)[2], bool force, int (&first)[2], int g) {
+    float m[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
-            if (force || m[i] * gdn_exp2i(-e[i]) > 16384.f) {
-                const int n = gdn_exp(m[i]) - 8;
-                e[i] = n < -100 ? -100 : n;
+        for (int c = 0; c < 2; ++c) m[c] = max3_abs_nan(m[c], x[i][c], x[i][c + 2]);
+    if (!gdn_exp_moves(m, e, force)) return;
+    if (__any_sync(0xffffffffu, !(m[0] <= kGdnFinite) || !(m[1] <= kGdnFinite))) {
+        m[0] = m[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (!(fabsf(x[i][c]) <= kGdnFinite)) {
+                    first[c & 1] = min(first[c & 1], 16 * i + g + (c >> 1) * 8);
+                    x[i][c] = 0.f;
+                }
+                m[c & 1] = fmaxf(m[c & 1], fabsf(x[i][c]));
             }
-        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) first[c] = min(first[c], __shfl_xor_sync(0xffffffffu, first[c], o));
     }
+    gdn_move_exp(m, e, force);
 }
 
 // Accumulator layout (rows g, g + 8 of each 16-row tile; columns 2*t4, 2*t4 + 1) to the second operand's (16 rows
@@ -625,6 +718,7 @@ struct GdnHandOver {
     uint4 s[HD / 16][32];
     float4 d[4][32];
     float2 s_up[32];
+    int2 first_bad[32];  // the first rows of a lane's two columns from which o is NaN, 64 for none
 };
 // All of a scan CTA's shared memory; the launch asks for its size, so no part of it can lie outside.
 template <typename T, int HD>
@@ -738,6 +832,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
                 d[i][3] = y.w;
             }
             const float2 su = hand.s_up[lane];
+            const int2 first_bad = hand.first_bad[lane];
             named_bar_arrive(kBarTaken + pair, 64);
             float o[4][4];
 #pragma unroll
@@ -787,6 +882,14 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
                     }
                 }
             }
+            if (min(first_bad.x, first_bad.y) < 64) {  // over what was stored
+#pragma unroll 1
+                for (int r = g; r < 64 && tok0 + r < p.t1; r += 8) {
+                    T* const dst = static_cast<T*>(a.o) + (tok0 + r) * a.o_row + h * HD + col;
+                    if (r >= first_bad.x) dst[0] = (T)__int_as_float(0x7FC00000);
+                    if (r >= first_bad.y) dst[1] = (T)__int_as_float(0x7FC00000);
+                }
+            }
         }
         return;
     }
@@ -799,6 +902,8 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
         for (int c = 0; c < 4; ++c)
             s[i][c] = p.state_in != nullptr ? sin[(c & 1) * HD + 16 * i + g + (c >> 1) * 8] : 0.f;
     int es[2] = {0, 0}, ex[2] = {0, 0}, ec[2] = {0, 0};
+    bool was_bad = false;
+    hand.first_bad[lane] = make_int2(64, 64);
     for (int ch = 0; ch < chunks; ++ch) {
         named_bar_sync(kBarReady, 160);
         const Stage& z = st[ch & 1];
@@ -839,7 +944,8 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
         }
         // d = T X
         uint32_t xh[4][2], xl[4][2];
-        gdn_col_exp(x, ex, force);
+        int first_bad[2] = {64, 64};
+        gdn_clean_exp(x, ex, force, first_bad, g);
         gdn_operand(x, ex, xh, xl);
         const float xu[2] = {gdn_exp2i(ex[0]) * z.d.t_up, gdn_exp2i(ex[1]) * z.d.t_up};
         float d[4][4];
@@ -858,6 +964,9 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) hand.d[i][lane] = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
+        const bool bad = min(first_bad[0], first_bad[1]) < 64;
+        if (bad || was_bad) hand.first_bad[lane] = make_int2(first_bad[0], first_bad[1]);
+        was_bad = bad;
         named_bar_arrive(kBarHand + pair, 64);
         // S <- e^G S + K^T (c d)
 #pragma unroll
@@ -868,7 +977,11 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
         gdn_col_exp(d, ec, force);
         gdn_operand(d, ec, dh, dl);
         const float cu[2] = {gdn_exp2i(ec[0]), gdn_exp2i(ec[1])};
-        const float decay = z.d.decay;
+        float decay[2] = {z.d.decay, z.d.decay};
+        if (bad) {
+            if (first_bad[0] < 64) decay[0] = __int_as_float(0x7FC00000);
+            if (first_bad[1] < 64) decay[1] = __int_as_float(0x7FC00000);
+        }
         const int krow = (lane & 7) + ((lane >> 4) << 3), kcol = ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int i = 0; i < kM; i += 2) {
@@ -890,7 +1003,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    s[i + e][c] = fmaf(decay, s[i + e][c], cu[c & 1] * fmaf(nl[e][c], 1.f / kGdnLo, nh[e][c]));
+                    s[i + e][c] = fmaf(decay[c & 1], s[i + e][c], cu[c & 1] * fmaf(nl[e][c], 1.f / kGdnLo, nh[e][c]));
         }
     }
     float* const sout = a.state_out + ((int64_t)h * HD + col) * HD;
