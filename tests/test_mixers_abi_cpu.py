@@ -189,3 +189,100 @@ def test_attn_workspace_bound_for_every_length(wz):
                 assert n <= 18944 * (4 * hd + 8) + 16, (T, qh, kvh, hd)
             worst = max(worst, n)
     assert worst > 18000 * (4 * 256 + 8)  # and it is not a loose one
+
+
+class DeviceTensor:
+    """A tensor's face on a device that need not be there."""
+
+    def __init__(self, dtype, shape, device):
+        self.dtype, self.shape, self.device_ = dtype, torch.Size(shape), device
+        self.is_cuda, self.nbytes = device >= 0, 1 << 40
+
+    def get_device(self):
+        return self.device_
+
+    def stride(self):
+        return torch.empty(self.shape, device="meta").stride()
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return A16
+
+
+class DeviceStream:
+    def __init__(self, device):
+        self.device_index, self.cuda_stream = device, 0x77
+
+
+@pytest.fixture
+def calls(wz, monkeypatch):
+    """The bindings over a library that notes the device and the stream of a call; device 0 is the current one."""
+    import contextlib
+    import types
+
+    now, seen = [0], []
+
+    @contextlib.contextmanager
+    def on_device(i):
+        before, now[0] = now[0], i
+        yield
+        now[0] = before
+
+    def entry(*args):
+        seen.append((now[0], args[-1]))
+        return 0
+
+    names = [f"wzyb_{n}_{t}" for n in ("kv_attn", "kv_tree_attn", "gdn_delta_rule") for t in ("f16", "f32")]
+    wz._torch_names()
+    monkeypatch.setattr(wz, "lib", lambda: types.SimpleNamespace(**{n: entry for n in names}))
+    monkeypatch.setattr(wz, "_current_raw_stream", lambda i: 100 + i)
+    monkeypatch.setattr(wz, "_current_device", lambda: now[0], raising=False)
+    monkeypatch.setattr(wz, "_on_device", on_device, raising=False)
+    return seen
+
+
+def mixer_calls(wz, where, stream=None):
+    """One call of each binding; where(name): the device of that argument."""
+    f, i, u = torch.float32, torch.int32, torch.uint8
+
+    def t(name, dtype, *shape):
+        return DeviceTensor(dtype, shape, where(name))
+
+    kw = dict(stream=stream, workspace=t("workspace", u, 1 << 20))
+    c = cache(wz)
+    a = dict(lse=t("lse", f, 3, 4), d_base_pos=t("d_base_pos", i, 1), **kw)
+    yield lambda: wz.kv_attn(t("q", f, 3, 4, 64), t("out", f, 3, 4, 64), c, 1, 16, **a)
+    yield lambda: wz.kv_tree_attn(t("q", f, 3, 4, 64), t("out", f, 3, 4, 64), c, c, t("mask", i, 3, 1), 1, 16, t("depth", i, 3), **a)
+    yield lambda: wz.gdn_delta_rule(t("q", f, 3, 2, 64), t("k", f, 3, 2, 64), t("v", f, 3, 4, 64), t("g", f, 3, 4), t("beta", f, 3, 4),
+                                    t("o", f, 3, 4, 64), t("state_out", f, 4, 64, 64), state_in=t("state_in", f, 4, 64, 64),
+                                    state_snaps=t("state_snaps", f, 3, 4, 64, 64), **kw)
+
+
+@pytest.mark.parametrize("device", [0, 1])
+def test_wrappers_launch_on_qs_device(wz, calls, device):
+    for run in mixer_calls(wz, lambda name: device):
+        run()
+    assert calls == [(device, 100 + device)] * 3
+    for run in mixer_calls(wz, lambda name: device, DeviceStream(device)):
+        run()
+    assert calls[3:] == [(device, 0x77)] * 3
+    for run in mixer_calls(wz, lambda name: device, DeviceStream(1 - device)):
+        with pytest.raises(ValueError):
+            run()
+    assert len(calls) == 6
+
+
+@pytest.mark.parametrize("other", ["out", "lse", "d_base_pos", "workspace", "mask", "depth", "k", "v", "g", "beta", "o", "state_in",
+                                   "state_out", "state_snaps"])
+@pytest.mark.parametrize("device", [-1, 1])
+def test_wrappers_refuse_tensors_of_two_devices(wz, calls, other, device):
+    users = {"out": 2, "lse": 2, "d_base_pos": 2, "workspace": 3}.get(other, 1)
+    refused = 0
+    for run in mixer_calls(wz, lambda name: device if name == other else 0):
+        try:
+            run()
+        except ValueError:
+            refused += 1
+    assert refused == users and len(calls) == 3 - users

@@ -474,22 +474,30 @@ def k_rope_kv_append(k, k_gamma, v, cos_tab, sin_tab, T, kv_heads, head_dim, cac
         call("wzyb_k_rope_kv_append_f16" if f16 else "wzyb_k_rope_kv_append_f32", *args)
 
 
-def _raw_stream(stream, index):
-    """The cudaStream_t of `stream`, or of the current stream of device `index`."""
-    return _current_raw_stream(index) if stream is None else stream.cuda_stream
+def _stream_on(stream, index):
+    """The cudaStream_t of `stream`, which has to be one of device `index`."""
+    if stream.device_index != index:
+        raise ValueError("stream: expected one of q's device")
+    return stream.cuda_stream
+
+
+def _call_on(index, fn, *args):
+    with _on_device(index):
+        return fn(*args)
 
 
 def _torch_names():
-    """torch's float16, float32, int32 and current-stream query, looked up once (a decoded token's calls are
-    short enough for repeated imports and attribute chains to show)."""
-    global _f16, _f32, _i32, _current_raw_stream
+    """torch's float16, float32, int32 and its queries of the current stream and device, looked up once (a decoded
+    token's calls are short enough for repeated imports and attribute chains to show)."""
+    global _f16, _f32, _i32, _current_raw_stream, _current_device, _on_device
     import torch
 
     _f16, _f32, _i32 = torch.float16, torch.float32, torch.int32
     _current_raw_stream = torch._C._cuda_getCurrentRawStream
+    _current_device, _on_device = torch._C._cuda_getDevice, torch.cuda.device
 
 
-_f16 = _f32 = _i32 = _current_raw_stream = None
+_f16 = _f32 = _i32 = _current_raw_stream = _current_device = _on_device = None
 
 
 def kv_attn_workspace_bytes(T, q_heads, kv_heads, head_dim) -> int:
@@ -500,30 +508,30 @@ def kv_attn_workspace_bytes(T, q_heads, kv_heads, head_dim) -> int:
 def _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace):
     if _f16 is None:
         _torch_names()
-    dt, shape = q.dtype, q.shape
-    if not (q.is_cuda and (dt is _f16 or dt is _f32) and len(shape) == 3):
+    dt, shape, dev = q.dtype, q.shape, q.get_device()  # a host tensor's device is -1
+    if not (dev >= 0 and (dt is _f16 or dt is _f32) and len(shape) == 3):
         raise ValueError("q: expected a float16 or float32 [T, q_heads, head_dim] tensor on a CUDA device")
     T, q_heads, head_dim = shape
     qr, qh, qe = q.stride()
     orow, oh, oe = out.stride()
-    if not (out.dtype is dt and out.shape == shape and out.is_cuda and qe == 1 and oe == 1):
+    if not (out.dtype is dt and out.shape == shape and out.get_device() == dev and qe == 1 and oe == 1):
         raise ValueError("out: expected q's shape, type and device, and both contiguous in the head dimension")
     lse_at = pos_at = ws_at = ws_bytes = 0
     if lse is not None:
-        if not (lse.dtype is _f32 and lse.shape == (T, q_heads) and lse.is_cuda and lse.is_contiguous()):
-            raise ValueError("lse: expected a contiguous float32 [T, q_heads] tensor on the device")
+        if not (lse.dtype is _f32 and lse.shape == (T, q_heads) and lse.get_device() == dev and lse.is_contiguous()):
+            raise ValueError("lse: expected a contiguous float32 [T, q_heads] tensor on q's device")
         lse_at = lse.data_ptr()
     if d_base_pos is not None:
-        if not (d_base_pos.dtype is _i32 and d_base_pos.is_cuda):
-            raise ValueError("d_base_pos: expected int32 on the device")
+        if not (d_base_pos.dtype is _i32 and d_base_pos.get_device() == dev):
+            raise ValueError("d_base_pos: expected int32 on q's device")
         pos_at = d_base_pos.data_ptr()
     if workspace is not None:
-        if not (workspace.is_cuda and workspace.is_contiguous()):
-            raise ValueError("workspace: expected a contiguous tensor on the device")
+        if not (workspace.get_device() == dev and workspace.is_contiguous()):
+            raise ValueError("workspace: expected a contiguous tensor on q's device")
         ws_at, ws_bytes = workspace.data_ptr(), workspace.nbytes
     return _KV_ATTN_PACK(q.data_ptr(), q_heads, qh, qr, out.data_ptr(), oh, orow, lse_at, ctypes.addressof(cache), source,
                          kv_heads, head_dim, pos_at, pos_offset, window, sinks,
-                         head_dim**-0.5 if scale is None else scale, ws_at, ws_bytes), T
+                         head_dim**-0.5 if scale is None else scale, ws_at, ws_bytes), T, dev
 
 
 def kv_attn(q, out, cache: KvCache, kv_heads, window, sinks=0, scale=None, source=KV_RING, d_base_pos=None,
@@ -531,9 +539,11 @@ def kv_attn(q, out, cache: KvCache, kv_heads, window, sinks=0, scale=None, sourc
     """Attention of the T tokens of q [T, q_heads, head_dim] (fp16 or fp32, any head and token stride) over the
     INT8 cache they were appended to: each sees the last `window` positions up to its own and the first
     `sinks`. scale defaults to head_dim**-0.5; workspace: kv_attn_workspace_bytes(...) bytes on the device."""
-    args, T = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    args, T, dev = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
     L = lib()
-    rc = (L.wzyb_kv_attn_f16 if q.dtype is _f16 else L.wzyb_kv_attn_f32)(args, T, _raw_stream(stream, q.get_device()))
+    fn = L.wzyb_kv_attn_f16 if q.dtype is _f16 else L.wzyb_kv_attn_f32
+    raw = _current_raw_stream(dev) if stream is None else _stream_on(stream, dev)
+    rc = fn(args, T, raw) if _current_device() == dev else _call_on(dev, fn, args, T, raw)
     if rc:
         check("wzyb_kv_attn", rc)
 
@@ -543,14 +553,16 @@ def kv_tree_attn(q, out, cache: KvCache, drafts: KvCache, mask, kv_heads, window
     """Attention of drafted nodes q [N, q_heads, head_dim]: node i stands at base + depth[i] over the `base`
     committed tokens of the cache and sees the drafts whose bit is set in mask [N, ceil(N / 32)] (int32 words);
     the drafts' k, v are cells 0..N-1 of the `drafts` ring."""
-    args, n = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
-    if not (mask.dtype is _i32 and mask.shape == (n, (n + 31) // 32) and mask.is_cuda and mask.is_contiguous()):
-        raise ValueError("mask: expected a contiguous int32 [N, ceil(N / 32)] tensor on the device")
-    if not (depth.dtype is _i32 and depth.shape == (n,) and depth.is_cuda and depth.is_contiguous()):
-        raise ValueError("depth: expected a contiguous int32 [N] tensor on the device")
+    args, n, dev = _kv_attn_pack(q, out, cache, kv_heads, window, sinks, scale, source, d_base_pos, pos_offset, lse, workspace)
+    if not (mask.dtype is _i32 and mask.shape == (n, (n + 31) // 32) and mask.get_device() == dev and mask.is_contiguous()):
+        raise ValueError("mask: expected a contiguous int32 [N, ceil(N / 32)] tensor on q's device")
+    if not (depth.dtype is _i32 and depth.shape == (n,) and depth.get_device() == dev and depth.is_contiguous()):
+        raise ValueError("depth: expected a contiguous int32 [N] tensor on q's device")
     L = lib()
-    rc = (L.wzyb_kv_tree_attn_f16 if q.dtype is _f16 else L.wzyb_kv_tree_attn_f32)(
-        args, ctypes.addressof(drafts), mask.data_ptr(), depth.data_ptr(), n, _raw_stream(stream, q.get_device()))
+    fn = L.wzyb_kv_tree_attn_f16 if q.dtype is _f16 else L.wzyb_kv_tree_attn_f32
+    raw = _current_raw_stream(dev) if stream is None else _stream_on(stream, dev)
+    rest = args, ctypes.addressof(drafts), mask.data_ptr(), depth.data_ptr(), n, raw
+    rc = fn(*rest) if _current_device() == dev else _call_on(dev, fn, *rest)
     if rc:
         check("wzyb_kv_tree_attn", rc)
 
@@ -567,37 +579,39 @@ def gdn_delta_rule(q, k, v, g, beta, o, state_out, state_in=None, state_snaps=No
     state_snaps [T, v_heads, d, d]: the state after every token. scale defaults to d**-0.5."""
     if _f16 is None:
         _torch_names()
-    dt, qk, vo = q.dtype, q.shape, v.shape
-    if not (q.is_cuda and (dt is _f16 or dt is _f32) and len(qk) == 3 and k.dtype is dt and k.shape == qk and k.is_cuda):
-        raise ValueError("q, k: expected float16 or float32 [T, k_heads, d] tensors on a CUDA device")
+    dt, qk, vo, dev = q.dtype, q.shape, v.shape, q.get_device()  # a host tensor's device is -1
+    if not (dev >= 0 and (dt is _f16 or dt is _f32) and len(qk) == 3 and k.dtype is dt and k.shape == qk and k.get_device() == dev):
+        raise ValueError("q, k: expected float16 or float32 [T, k_heads, d] tensors on one CUDA device")
     T, k_heads, d = qk
-    if not (v.dtype is dt and len(vo) == 3 and vo[0] == T and vo[2] == d and v.is_cuda and o.dtype is dt and o.shape == vo
-            and o.is_cuda):
-        raise ValueError("v, o: expected [T, v_heads, d] tensors of q's type on the device")
+    if not (v.dtype is dt and len(vo) == 3 and vo[0] == T and vo[2] == d and v.get_device() == dev and o.dtype is dt and o.shape == vo
+            and o.get_device() == dev):
+        raise ValueError("v, o: expected [T, v_heads, d] tensors of q's type on q's device")
     v_heads = vo[1]
     (qr, qh, qe), (kr, kh, ke), (vr, vh, ve), (orow, oh, oe) = q.stride(), k.stride(), v.stride(), o.stride()
     if not (qe == ke == ve == oe == 1 and (k_heads == 1 or qh == kh == d) and (v_heads == 1 or vh == oh == d)):
         raise ValueError("q, k, v, o: the heads of a token must be contiguous")
     th, st = (T, v_heads), (v_heads, d, d)
-    if not (g.dtype is _f32 and beta.dtype is _f32 and g.shape == th and beta.shape == th and g.is_cuda and beta.is_cuda
+    if not (g.dtype is _f32 and beta.dtype is _f32 and g.shape == th and beta.shape == th and g.get_device() == dev and beta.get_device() == dev
             and g.is_contiguous() and beta.is_contiguous()):
-        raise ValueError("g, beta: expected contiguous float32 [T, v_heads] tensors on the device")
+        raise ValueError("g, beta: expected contiguous float32 [T, v_heads] tensors on q's device")
     at = [0, 0, 0]
     for i, (t, shape) in enumerate(((state_in, st), (state_out, st), (state_snaps, (T, v_heads, d, d)))):
         if t is not None:
-            if not (t.dtype is _f32 and t.shape == shape and t.is_cuda and t.is_contiguous()):
-                raise ValueError("states: expected contiguous float32 [v_heads, d, d] (snapshots [T, v_heads, d, d]) on the device")
+            if not (t.dtype is _f32 and t.shape == shape and t.get_device() == dev and t.is_contiguous()):
+                raise ValueError("states: expected contiguous float32 [v_heads, d, d] (snapshots [T, v_heads, d, d]) on q's device")
             at[i] = t.data_ptr()
     ws_at = ws_bytes = 0
     if workspace is not None:
-        if not (workspace.is_cuda and workspace.is_contiguous()):
-            raise ValueError("workspace: expected a contiguous tensor on the device")
+        if not (workspace.get_device() == dev and workspace.is_contiguous()):
+            raise ValueError("workspace: expected a contiguous tensor on q's device")
         ws_at, ws_bytes = workspace.data_ptr(), workspace.nbytes
     args = _GDN_DELTA_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), qr, kr, vr, g.data_ptr(), beta.data_ptr(), *at,
                            o.data_ptr(), orow, k_heads, v_heads, d, d**-0.5 if scale is None else scale,
                            1 if qk_l2norm else 0, l2_eps, ws_at, ws_bytes)
     L = lib()
-    rc = (L.wzyb_gdn_delta_rule_f16 if dt is _f16 else L.wzyb_gdn_delta_rule_f32)(args, T, _raw_stream(stream, q.get_device()))
+    fn = L.wzyb_gdn_delta_rule_f16 if dt is _f16 else L.wzyb_gdn_delta_rule_f32
+    raw = _current_raw_stream(dev) if stream is None else _stream_on(stream, dev)
+    rc = fn(args, T, raw) if _current_device() == dev else _call_on(dev, fn, args, T, raw)
     if rc:
         check("wzyb_gdn_delta_rule", rc)
 
