@@ -755,3 +755,24 @@ def test_gdn_infinities_and_nan_reach_no_earlier_token(wz, dtype, T, l2, bad, wh
         spoiled_o[at:, heads] = spoiled_s[heads] = True
     assert torch.equal(o[~spoiled_o], clean[0][~spoiled_o]) and torch.equal(s[~spoiled_s], clean[1][~spoiled_s])
     assert not torch.isfinite(o[spoiled_o]).any() and not torch.isfinite(s[spoiled_s]).any()
+
+
+@pytest.mark.parametrize("T", [2, 40])
+@pytest.mark.parametrize("size", [2.0**-140, 2.0**-60, 2.0**60, 2.0**119, 2.0**122])
+def test_attn_query_sizes_over_fp32s_range(wz, T, size):
+    """Scores far below 1 weigh all cells alike, scores far above 1 take the largest alone; nothing overflows on the way as
+    long as the scores themselves are fp32 numbers (they reach 8 times the query's largest element here, at most)."""
+    r = gen(27)
+    n, hd = 64, 64
+    rows, _, desc = make_cache(wz, n, 16, n, hd, r, True)
+    q = torch.randn(T, 4, hd, generator=r, device=DEV) * size
+    out, lse = torch.zeros_like(q), torch.zeros(T, 4, device=DEV)
+    wz.kv_attn(q, out, desc, 1, n, source=wz.KV_FULL, pos_offset=n - T, lse=lse, workspace=workspace(wz, T, 4, 1, hd))
+    o, wl, mag, _ = ref.attention(q, rows, 1, hd, hd**-0.5, [list(range(n - T + t + 1)) for t in range(T)])
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    assert ((lse.double() - wl).abs() <= wl.abs() * 2.0**-16 + 2.0**-18).all()
+    if size < 1:
+        assert ((out.double() - o).abs() <= mag * 2.0**-19).all()
+    else:  # one cell's value, unless two scores are as close as their own error
+        v = ref.rows64(rows[2], rows[3], hd, 0)
+        assert ((out.double().unsqueeze(2) - v).abs().amax(-1).amin(-1) <= 2.0**-20 * v.abs().max()).all()

@@ -229,6 +229,9 @@ __device__ __forceinline__ int scale_exp(float x) {
     const uint32_t e = b >> 23;  // scales are >= 0; a set sign bit lands outside [1, 254]
     return e >= 1 && e <= 254 ? (int)e - 126 : -1000;
 }
+// The exponent by which a query row is scaled down, from its largest magnitude's: rows whose scores are 0 either way, and
+// infinite or NaN ones (-1000), as they are; 2^-e stays a normal number.
+__device__ __forceinline__ int row_exp(int e) { return e < -100 ? 0 : (e > 126 ? 126 : e); }
 __device__ __forceinline__ float exp2_int(int e) {  // 2^e, 0 below the normal range
     return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
@@ -260,7 +263,7 @@ __device__ __forceinline__ void stage_rows(const KvAttnArgs& a, int head, int ro
             for (int i = 0; i < kE; ++i) am = fmaxf(am, fabsf(x[i]));
             am = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
             int e = scale_exp(am);
-            if (e < -100 || e > 120) e = 0;
+            e = row_exp(e);
             const float down = exp2_int(-e);
             f *= exp2_int(e);
 #pragma unroll
@@ -846,7 +849,7 @@ __global__ void __launch_bounds__(TcSmem<T, HD, kReg>::kThreads, 1) kv_attn_tile
 #pragma unroll
                     for (int o = kL / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
                     int e = scale_exp(am);
-                    if (e < -100 || e > 120) e = 0;
+                    e = row_exp(e);
                     const float down = exp2_int(-e);
                     uint32_t h[4], l[4];
 #pragma unroll
