@@ -776,3 +776,18 @@ def test_attn_query_sizes_over_fp32s_range(wz, T, size):
     else:  # one cell's value, unless two scores are as close as their own error
         v = ref.rows64(rows[2], rows[3], hd, 0)
         assert ((out.double().unsqueeze(2) - v).abs().amax(-1).amin(-1) <= 2.0**-20 * v.abs().max()).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T", [90, 400])
+def test_gdn_fp16_outputs_are_rounded_once(wz, hd, T):
+    """An fp16 call computes as the fp32 call on the same numbers does and rounds its outputs at the end. The two calls'
+    results before that are within 2^-18 of each other (relative to the output's size, 22-bit parts and their sums), so a
+    share of 2 * 2^-18 / 2^-11 of the roundings may fall the other way, and those by one step."""
+    r = gen(28)
+    q, k, v, g, beta, s0 = gdn_inputs(T, 2, 4, hd, torch.float16, r, False, True)
+    o16, s16 = gdn_call(wz, q, k, v, g, beta, s0)
+    o32, s32 = gdn_call(wz, q.float(), k.float(), v.float(), g, beta, s0)
+    off = o16 != o32.half()
+    assert off.double().mean() <= 2.0**-6
+    assert ((o16.float() - o32).abs() <= 2.0**-10 * o32.abs() + 2.0**-24).all()

@@ -219,10 +219,9 @@ constexpr float kGdnFinite = 3.402823466e38f;  // the largest finite number: nei
 
 // A (chunk, value head)'s part of the workspace. Matrices as mma A fragments, 16 bytes per lane: fragment
 // (m-tile i, k-step j <= i) at index i * (i + 1) / 2 + j, 512 bytes each.
-template <bool kSplit>
 struct GdnChunkData {
     uint4 t_hi[10][32], t_lo[10][32];
-    uint4 p[kSplit ? 20 : 10][32];  // split: hi parts, then lo parts
+    uint4 p[20][32];  // hi parts, then lo parts
     float a[64], b[64], c[64];      // row factors of K S, Q S and d
     float decay, t_up, p_up, pad;   // e^(G_64), 2^e of T and of P
 };
@@ -430,8 +429,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
     if (warp == 0) load_gb(hk * per);
     for (int hv = 0; hv < per; ++hv) {
         const int h = hk * per + hv;
-        GdnChunkData<kSplit>& out =
-            reinterpret_cast<GdnChunkData<kSplit>*>(p.data)[(int64_t)chunk * a.v_heads + h];
+        GdnChunkData& out = reinterpret_cast<GdnChunkData*>(p.data)[(int64_t)chunk * a.v_heads + h];
         if (warp == 0) {
             // running sums in fp64, held as two fp32 parts in log2 units: differences of close tokens keep their
             // precision after strong decays. A decay below e^-120 is 0 in fp32 either way (so -inf is as well).
@@ -602,7 +600,7 @@ __global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p
                 gdn_split(pv[2 * j + b][2] * pd, pv[2 * j + b][3] * pd, h[2 * b + 1], l[2 * b + 1]);
             }
             out.p[at][lane] = make_uint4(h[0], h[1], h[2], h[3]);
-            if constexpr (kSplit) out.p[10 + at][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+            out.p[10 + at][lane] = make_uint4(l[0], l[1], l[2], l[3]);
         }
         if (tid == 0) {
             out.decay = sm.first_bad < 64 ? __int_as_float(0x7FC00000) : ex2_approx(sm.ghi[63] + sm.glo[63]);
@@ -627,7 +625,7 @@ struct GdnScanStage {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr int kLd = HD + 8, kVLd = 32 + 16 / sizeof(T);
     GdnKq<kSplit, HD> kq;
-    GdnChunkData<kSplit> d;
+    GdnChunkData d;
     T v[64 * kVLd];
 };
 
@@ -788,7 +786,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
             if (ch == chunks) break;
             Stage& s = st[ch & 1];
             if (lane == 0 && lost < 0) {
-                constexpr int kKq = sizeof(GdnKq<kSplit, HD>), kData = sizeof(GdnChunkData<kSplit>);
+                constexpr int kKq = sizeof(GdnKq<kSplit, HD>), kData = sizeof(GdnChunkData);
                 mbar_arrive_expect_tx(&full[ch & 1], kKq + kData);
                 bulk_load(&s.kq, p.kq + ((int64_t)ch * a.k_heads + hk) * kKq, kKq, &full[ch & 1], policy);
                 bulk_load(&s.d, p.data + ((int64_t)ch * a.v_heads + h) * kData, kData, &full[ch & 1], policy);
@@ -866,7 +864,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
                     const uint4 ph = z.d.p[i * (i + 1) / 2 + j][lane];
                     mma_f16(oh, ph, dh[j][0], dh[j][1]);
                     mma_f16(ol, ph, dl[j][0], dl[j][1]);
-                    if constexpr (kSplit) mma_f16(ol, z.d.p[(kSplit ? 10 : 0) + i * (i + 1) / 2 + j][lane], dh[j][0], dh[j][1]);
+                    mma_f16(ol, z.d.p[10 + i * (i + 1) / 2 + j][lane], dh[j][0], dh[j][1]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[i][c] = fmaf(c & 1 ? up.y : up.x, fmaf(ol[c], 1.f / kGdnLo, oh[c]), o[i][c]);
@@ -1017,8 +1015,7 @@ __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArg
 constexpr int64_t kGdnSegBytes = int64_t(96) << 20;
 static int64_t gdn_chunk_bytes(bool f32, int k_heads, int v_heads, int head_dim) {
     const int64_t row = 2 * 64 * (head_dim + 8) * (int64_t)sizeof(__half);  // of a GdnKq, K and Q
-    return f32 ? v_heads * (int64_t)sizeof(GdnChunkData<true>) + k_heads * 2 * row
-               : v_heads * (int64_t)sizeof(GdnChunkData<false>) + k_heads * row;
+    return v_heads * (int64_t)sizeof(GdnChunkData) + k_heads * (f32 ? 2 * row : row);
 }
 static int64_t gdn_most_chunks(bool f32, int64_t T, int k_heads, int v_heads, int head_dim) {
     const int64_t n = kGdnSegBytes / gdn_chunk_bytes(f32, k_heads, v_heads, head_dim), all = (T + kGdnChunk - 1) / kGdnChunk;
@@ -1049,7 +1046,7 @@ static int launch_gdn_chunked(const GdnDeltaArgs& a, uint8_t* ws, cudaStream_t s
     GdnScanArgs sa;
     pa.x = sa.x = a;
     pa.data = ws;
-    pa.kq = ws + seg * a.v_heads * (int64_t)sizeof(GdnChunkData<kSplit>);
+    pa.kq = ws + seg * a.v_heads * (int64_t)sizeof(GdnChunkData);
     sa.data = pa.data;
     sa.kq = pa.kq;
     sa.state_in = a.state_in;
