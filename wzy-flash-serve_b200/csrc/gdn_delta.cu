@@ -299,8 +299,16 @@ __device__ __noinline__ void gdn_zero_bad_k(const GdnPrepArgs& p, GdnPrepSmem<T,
 // sums at 3 CTAs per SM (168 registers): 64 chunks of 16/32 heads of 128, fp16, 73 us, a quarter of the call's time.
 // Halving (the 64 rows as 32 + 32, those as 16 + 16) has longer sums and shorter chains, but needs 209 registers: 2 CTAs
 // per SM, 6 % slower.
+// The least CTAs per SM that the registers have to leave room for (0: the compiler's choice, which is 168 registers too):
+// shared memory holds two of fp32 with head_dim 128. us at 8192 tokens of 16/32 (fp32: 16/48) heads: fp32, 128: 1148 with
+// two, 1193 with the compiler's choice; fp16, 128: 490 with its choice, 496 with three (more spills), 506 with one; fp16,
+// 64: 391 with three, 414 with its choice (172 registers); fp32, 64: 536 and 580.
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) gdn_chunk_prep_kernel(const GdnPrepArgs p) {
+constexpr int gdn_prep_ctas() {
+    return HD == 64 ? 3 : (sizeof(T) == 4 ? 2 : 0);
+}
+template <typename T, int HD>
+__global__ void __launch_bounds__(128, gdn_prep_ctas<T, HD>()) gdn_chunk_prep_kernel(const GdnPrepArgs p) {
     pdl_begin();
     using S = GdnPrepSmem<T, HD>;
     constexpr bool kSplit = S::kSplit;
