@@ -14,7 +14,8 @@
  *    device memory from the host, so every launcher may be recorded into a CUDA graph by stream
  *    capture (call wzyb_prepare_device() once per device before the first capture).
  *  - fp16 tensors are passed as uint16_t* (IEEE binary16 bit patterns, i.e. __half storage);
- *    fp32 tensors as float*. Arithmetic is fp32; fp16 outputs are rounded to nearest-even once.
+ *    fp32 tensors as float*. Arithmetic is fp32; fp16 outputs are rounded to nearest-even once
+ *    (the _f16 attention calls also round the softmax weights to fp16, see there).
  *  - Row-major layouts; every row / head start must be 16-byte aligned (checked).
  *  - The kernel is enqueued on `stream` (a cudaStream_t) of the CURRENT device; the caller sets the
  *    device, as StageGpu does with cudaSetDevice(dev).
@@ -487,9 +488,13 @@ int wzyb_embed_ple_f16(const wzyb_embed_ple_args* a, int64_t T, wzyb_stream_t st
  *   x_j = scale * (q . k_j);  out = sum_j softmax(x)_j v_j;  lse[t, h] = ln sum_j exp(x_j)  (lse may be NULL)
  * with k_j, v_j = code * scale of the cell's 64-element groups. A query that sees nothing gets out = 0 and
  * lse = -inf. Cells that a query does not see never reach its result, whatever they hold.
+ * Precision: scores, maxima and sums are fp32. The _f32 calls take q and the weights p_j * (v's scale) as two fp16
+ * parts (22 bits); the _f16 calls round each weight to fp16 (2^-12 of it at most, as much as the output's own
+ * rounding), and may sum up to 16,384 keys in the tensor cores, which cut off at 2^-23 per 16 keys.
  * head_dim in {64, 128, 256}; q_heads a multiple of kv_heads, at most 256; kv_heads <= 64; T <= 2^22 (0: nothing to
  * do, the per-token pointers may be NULL);
- * max_ctx and ring_cap at most 2^30; strides in elements. Cache codes and scales 16-byte aligned.
+ * max_ctx and ring_cap at most 2^30; strides in elements, q's any >= 0, out's so that a token's heads do not overlap and
+ * lie before the next token's. q, out, their strides in bytes, cache codes and scales 16-byte aligned.
  * workspace: wzyb_kv_attn_workspace(T, q_heads, kv_heads, head_dim) bytes of device memory (0: none needed),
  * 16-byte aligned, of no meaning between calls; calls on different streams need their own. The size does not grow
  * with T (long calls need none): 18944 * (4 * head_dim + 8) + 16 bytes serve every T and every head count.
@@ -541,7 +546,8 @@ int wzyb_kv_tree_attn_f32(const wzyb_kv_attn_args* a, const wzyb_kv_cache* draft
  *   S <- e^(g_t) S;  d = beta_t (v_t - S k_t);  S <- S + d k_t^T;  o_t = scale * S q_t
  * q, k [T, k_heads, head_dim], v, o [T, v_heads, head_dim] (fp16 for _f16, fp32 for _f32; heads contiguous,
  * tokens *_row_stride elements apart, so q, k, v may be slices of one projection); g (log decay, usually
- * <= 0, -inf resets) and beta [T, v_heads] fp32. qk_l2norm != 0 norms q and k first:
+ * <= 0, -inf resets) and beta [T, v_heads] fp32. States and sums are fp32, products keep 22 bits, fp16 outputs are
+ * rounded once, whatever the sizes of scale, q and beta. qk_l2norm != 0 norms q and k first:
  * x * rsqrt(sum x^2 + l2_eps). state_in [v_heads, head_dim, head_dim] fp32 or NULL (zeros), state_out the
  * state after the last token (the same buffer as state_in is allowed); state_snaps [T, v_heads, head_dim,
  * head_dim] or NULL: the state after every token, for taking back rejected drafts. head_dim in {64, 128};

@@ -296,7 +296,7 @@ __device__ __noinline__ void gdn_zero_bad_k(const GdnPrepArgs& p, GdnPrepSmem<T,
 // One CTA of 4 warps per (chunk, k head), over the value heads that share it. Warp w owns rows 16w .. 16w+15.
 // T by blocks of 16: a diagonal block's inverse by forward substitution (a lane per column), then the column
 // block j below it by warp j: T_ij = -T_ii sum_k A_ik T_kj, fp32 FMA. Bound by the latency of those short dependent
-// sums at 3 CTAs per SM (168 registers): 64 chunks of 16/32 heads of 128, fp16, 73 us, a quarter of the call's time.
+// sums at 3 CTAs per SM (168 registers): 64 chunks of 16/32 heads of 128, fp16, 73 us, 30 % of the call's time.
 // Halving (the 64 rows as 32 + 32, those as 16 + 16) has longer sums and shorter chains, but needs 209 registers: 2 CTAs
 // per SM, 6 % slower.
 // The least CTAs per SM that the registers have to leave room for (0: the compiler's choice, which is 168 registers too):
@@ -749,8 +749,8 @@ __device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
 // output warp takes S and d from it when T X is done and makes o = e^G Q S + P d beside the rest of the chunk and the
 // start of the next one (one warp for both took 1.5 times as long). The CTA's four pairs share the chunk's K, Q, T and
 // P in shared memory; a ninth warp fetches the next chunk's meanwhile.
-// Bound: the state warp's chain per chunk of 64 tokens, 4700 cycles (fp16) or 6500 (fp32), the tensor pipe busy 49 % of
-// it. 16/32 heads of 128, fp16: 4096 tokens 171 us; 32,768 tokens with the prep 1851 us. One CTA per SM: 128 CTAs hold 32
+// Bound: the state warp's chain per chunk of 64 tokens, about 5000 cycles (fp16) or 6500 (fp32), the tensor pipe of an SM
+// that has a CTA busy 49 % of it. 16/32 heads of 128, fp16: 32,768 tokens with the prep 1900 us. One CTA per SM: 128 CTAs hold 32
 // heads; 48 heads are two waves.
 template <typename T, int HD>
 __global__ void __launch_bounds__(288, 1) gdn_chunk_scan_kernel(const GdnScanArgs p) {
@@ -1037,7 +1037,7 @@ static int64_t gdn_seg_chunks(bool f32, int64_t T, int k_heads, int v_heads, int
 }
 // Calls of at least this many tokens take the chunked form. Chunked / token by token, us per call: fp16 16/32 heads of
 // 128, 64 tokens 22 / 21, 96 26 / 30, 256 34 / 78; fp32 16/48 heads 64 tokens 38 / 32, 96 45 / 47; fp32 2/6 heads of
-// 64, 96 tokens 28 / 23, 128 28 / 31.
+// 64, 96 tokens 28 / 23, 128 28 / 31 (one rule for all: the smallest models lose up to 5 us there).
 constexpr int64_t kGdnChunkedFrom = 96;
 
 template <typename T, int HD>

@@ -7,8 +7,10 @@
 // Codes are integers up to 127, exact in fp16, so the tensor cores multiply the codes themselves and the
 // scales stay fp32: on the K side they multiply the per-group partial products, on the V side the softmax
 // weights (one scaled copy of the weights per group). Products accumulate in fp32, statistics are fp32.
-// The one rounding to fewer bits for fp16 calls is the scaled weight p * vs to fp16 (relative 2^-12 each,
-// the size of the output's own rounding); fp32 calls split q and p * vs into two fp16 parts (22 bits).
+// The one rounding to fewer bits for fp16 calls is the scaled weight p * vs to fp16 (2^-12 of each at most, the size
+// of the output's own rounding; error against 64 bits 2.9e-4 where the output's rounding alone gives 2.1e-4): a
+// second part, as fp32 calls have it, would double p V and the weights' work, 1100 of a tile's 4200 cycles. fp32 calls
+// split q and p * vs into two fp16 parts (22 bits).
 //
 // Weights entering the tensor cores are p * vs * 2^(7 - E) with a running E per row (from the largest finite
 // scale among the cells that the row sees, as the running maximum of its scores), so they sit in fp16's
@@ -652,8 +654,8 @@ __global__ void __launch_bounds__(128) kv_attn_few_kernel(const KvAttnArgs a) {
 // than kAttnDriftKeys, sum in registers; shorter fp16 calls in tensor memory, which is faster.
 // 64 keys per tile: the four groups' scores and the tile's p V then fill tensor memory, so a tile's products and its
 // softmax take turns, and that sum bounds the kernel. Measured with 16/2 heads of 256: 4096 fp16 tokens with a window
-// of 8192 in 1419 us, a tile 4200 cycles (scores 1000, softmax and weights 2700, p V 500); 64 fp32 nodes of 24/2 heads
-// over 131,072 cells in 755 us, a tile 6000 cycles (scores 2000, softmax with split weights 3600), kReg.
+// of 8192 in 1440 us, a tile 4200 cycles (scores 1000, softmax and weights 2700, p V 500); 64 fp32 nodes of 24/2 heads
+// over 131,072 cells in 738 us, a tile 5900 cycles (scores 2000, softmax with split weights 3500), kReg.
 // Every wait is bounded. A role whose wait gives up ends its loop; the others, which wait for it, run out beside it.
 // ----------------------------------------------------------------------------------------------------
 // Issued by one elected lane of a converged warp: the warp-uniform operands stay in uniform registers (inside an
